@@ -256,7 +256,8 @@ __global__ __launch_bounds__(kFrameBlock, GYMHIP_ATARI_WAVES) void atari_preproc
     // leave as one 4-B store.  VALU-lean on purpose (the kernel overlaps this phase with other workgroups' loads, and what it costs is
     // issue slots): an output column's x-taps are CONSECUTIVE source pixels (computeResizeAreaTab), so a column keeps one base index and
     // its taps are immediate offsets of the LDS reads (a padded tap reads the next pixel and multiplies it by its weight 0: adds +0);
-    // columns are processed in pairs with packed fp32 multiplies and adds (v_pk_mul_f32 / v_pk_add_f32: per lane the same IEEE
+    // columns are processed in pairs (two-wide vector types, compiled to scalar multiplies and adds: the Makefile turns packed fp32 off.
+    // MI355X, 4096 envs: RGB 0.158 ms against 0.159 with it, random index screens 0.120 against 0.117; per lane the same IEEE
     // operations in the same order as OpenCV's scalar loop); the horizontal sum starts from the first product rather than from 0 + product
     // (the products are >= +0, so 0 + p == p bit for bit); v_cvt_pk_u8_f32 is saturate_cast<uchar> (round half to even, clamp:
     // tools/cvt_probe.hip) and packs the byte in the same instruction. -----------------------------------------------------------------
