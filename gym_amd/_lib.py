@@ -21,6 +21,8 @@ WRAP_NO_AUTO_RESET = 64
 ACT_I32, ACT_I64, ACT_U8 = 0, 1, 2
 STACK_INTENDED, STACK_AS_WRITTEN = 0, 1
 OUT_F16, OUT_BF16 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+POLICY_MAX_WIDTH = 1 << 24
 NOALLOC_MAX_ROWS = 1 << 26
 
 
@@ -78,6 +80,45 @@ class AtariConfig(C.Structure):
     ]
 
 
+class LogitRules(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("history_dtype", C.c_int32),
+        ("history_len_dtype", C.c_int32),
+        ("reserved", C.c_int32),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_int64),
+        ("mask_lines", C.c_int64),
+        ("mask_rows", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("bias_stride", C.c_int64),
+        ("history", C.c_void_p),
+        ("history_stride", C.c_int64),
+        ("history_cols", C.c_int64),
+        ("history_len", C.c_void_p),
+        ("repetition_rows", C.c_void_p),
+        ("presence_rows", C.c_void_p),
+        ("frequency_rows", C.c_void_p),
+        ("temperature_rows", C.c_void_p),
+        ("repetition", C.c_float),
+        ("presence", C.c_float),
+        ("frequency", C.c_float),
+        ("temperature", C.c_float),
+    ]
+
+
+class RandomKeys(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("steps_per_row", C.c_int32),
+        ("seed", C.c_uint64),
+        ("row", C.c_int64),
+        ("step", C.c_int64),
+        ("rows", C.c_void_p),
+        ("steps", C.c_void_p),
+    ]
+
+
 # Every symbol include/gymhip.h declares: (restype, argtypes)
 _vp, _i64, _i32, _u64 = C.c_void_p, C.c_int64, C.c_int32, C.c_uint64
 SIGNATURES = {
@@ -132,6 +173,14 @@ SIGNATURES = {
     "gymhip_atari_set_stack_view": (C.c_int, [_vp, C.c_int]),
     "gymhip_atari_materialize_nchw_f32": (C.c_int, [_vp, _vp, _vp]),
     "gymhip_atari_materialize_nchw_16": (C.c_int, [_vp, _vp, C.c_int, _vp]),
+    "gymhip_process_logits": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "gymhip_process_logits_backward": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "gymhip_sample_workspace_bytes": (C.c_size_t, [_i64, _i64]),
+    "gymhip_sample_actions": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "gymhip_action_log_prob_workspace_bytes": (C.c_size_t, [_i64, _i64]),
+    "gymhip_action_log_prob": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _vp, C.c_int, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "gymhip_action_log_prob_backward": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _vp, C.c_int] + [_vp] * 6 + [_i64, _vp]),
+    "gymhip_dropout": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, C.c_double, _vp, _vp, _i64, _vp]),
 }
 
 _lib = None

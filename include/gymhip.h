@@ -349,6 +349,83 @@ int gymhip_host_env_post_step(int64_t n, const float* reward_in, const uint8_t* 
                               uint8_t* st_was_real_done, float* st_return, float* st_length, int clip_reward, float* reward_out,
                               uint8_t* done_out, uint8_t* has_episode, float* ep_return, float* ep_length, void* stream);
 
+/* ======================================================================================================================
+ * The policy's end of the VecEnv loop: logits to actions, their scores with gradients, dropout.  NO COUNTERPART IN THE REFERENCE
+ * (its trainer is outside the repository; VecEnv::step takes finished actions, base.h:56-63).  Stateless: every pointer is device
+ * memory of the CURRENT device, calls enqueue on `stream`, allocate nothing and may be recorded into a HIP graph; two calls at once
+ * need two workspaces.  rows = 0 is allowed and does nothing.
+ * ==================================================================================================================== */
+enum { GYMHIP_TYPE_F32 = 0, GYMHIP_TYPE_F16 = 1, GYMHIP_TYPE_BF16 = 2 };
+/* The widest row of logits or features.  Offsets are 64-bit: rows x stride is not limited. */
+#define GYMHIP_POLICY_MAX_WIDTH (1ll << 24)
+
+/* What is done to a row's logits x before anything is chosen or scored.  c = how often v occurs in the row's history:
+ *     x' = x, or where c > 0: (x > 0 ? x / repetition : x * repetition) - frequency * c - presence
+ *     z  = (x' + bias[v]) / temperature;   z = -inf where the mask's bit v is 0, whatever x holds there (NaN and infinities too)
+ * temperature 0: z is left undivided, and gymhip_sample_actions takes the greatest z, the lowest v among equal ones.
+ * Pointers may be NULL.  History ids outside [0, width) are skipped, so any padding value of that kind will do. */
+typedef struct gymhip_logit_rules {
+    int32_t struct_size;           /* = sizeof(gymhip_logit_rules) */
+    int32_t history_dtype;         /* GYMHIP_ACT_I32 or GYMHIP_ACT_I64 */
+    int32_t history_len_dtype;     /* likewise */
+    int32_t reserved;              /* 0 */
+    const uint32_t* mask;          /* [mask_lines] lines of ceil(width / 32) words; bit v % 32 of word v / 32 is 1 where v is allowed */
+    int64_t mask_stride;           /* words from one line to the next */
+    int64_t mask_lines;
+    const int32_t* mask_rows;      /* [rows] line of each row: negative = everything allowed, >= mask_lines = nothing allowed.
+                                      NULL: mask_lines is 1 (one line for all rows) or `rows` */
+    const float* bias;             /* row b's bias vector is bias + b * bias_stride; stride 0 = one for all rows */
+    int64_t bias_stride;
+    const void* history;           /* [rows][history_cols] ids of history_dtype */
+    int64_t history_stride, history_cols;
+    const void* history_len;       /* [rows] how many of a row's ids count (clamped to 0 .. history_cols); NULL = all */
+    const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows; /* [rows] each, or NULL = the value below */
+    float repetition, presence, frequency, temperature; /* neutral: 1, 0, 0, 1.  repetition > 0, temperature >= 0 */
+} gymhip_logit_rules;
+
+/* Random numbers are a function of (seed, row key, step) alone (Philox4x32 of Salmon et al. 2011 with 7 rounds): nothing is stored, any
+ * subset of rows in any order draws the same, and sharded ranks agree with one GPU when a row's key is the env's GLOBAL index.
+ * Keys and steps count modulo 2^48. */
+typedef struct gymhip_random_keys {
+    int32_t struct_size;           /* = sizeof(gymhip_random_keys) */
+    int32_t steps_per_row;         /* steps != NULL: 1 = [rows] steps, 0 = one step for all rows (a device word, so that a recorded
+                                      graph draws anew when the caller advances it) */
+    uint64_t seed;
+    int64_t row, step;             /* row key of row 0 (row b: row + b) and the step, where the pointers below are NULL */
+    const int64_t *rows, *steps;
+} gymhip_random_keys;
+
+/* z of `logits` [rows][width] (type, element stride between rows) rounded once to the same type.  `out` may be `logits` itself (same
+ * stride); any other overlap is GYMHIP_EINVAL. */
+int gymhip_process_logits(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules, void* out,
+                          int64_t out_stride, void* stream);
+/* d(logits) from d(z): 0 where the mask's bit is 0. */
+int gymhip_process_logits_backward(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                                   const void* grad_out, int64_t grad_out_stride, void* grad_in, int64_t grad_in_stride, void* stream);
+/* One action per row from softmax(z), and its log-probability: the least v whose running sum of exp(z - max z) passes u times the whole
+ * sum, u in (0, 1) from `keys`.  Decided in double precision, so that the action does not hang on how the row is split or summed.
+ * A row in which nothing is allowed (or every z is -inf) gives action -1 and log-probability -inf; one that holds a NaN or +inf among
+ * its allowed z gives -1 and NaN.  workspace: gymhip_sample_workspace_bytes(rows, width) bytes, 16-B aligned, contents free. */
+size_t gymhip_sample_workspace_bytes(int64_t rows, int64_t width);
+int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                          const gymhip_random_keys* keys, int32_t* actions, float* log_prob, void* workspace, size_t workspace_bytes, void* stream);
+/* log softmax(z)[action] and the entropy of softmax(z), float32 per row, and for the backward pass log_sum, double [rows][2]: max z and
+ * the logarithm of the sum of exp(z - max z), apart so that a row of the type's lowest values keeps the latter.  An action
+ * that is not allowed or outside [0, width) has -inf, and no gradient; a row in which nothing is allowed has -inf, entropy 0 and no
+ * gradient.  workspace as above. */
+size_t gymhip_action_log_prob_workspace_bytes(int64_t rows, int64_t width);
+int gymhip_action_log_prob(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                           const void* actions, int action_dtype, float* log_prob, float* entropy, double* log_sum, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* d(logits) from d(log_prob) and d(entropy) (either may be NULL = zeros). */
+int gymhip_action_log_prob_backward(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                                    const void* actions, int action_dtype, const float* log_prob, const float* entropy, const double* log_sum,
+                                    const float* grad_log_prob, const float* grad_entropy, void* grad_in, int64_t grad_in_stride, void* stream);
+/* y = x * 65536 / (65536 - t) where the element's 16 random bits are >= t = round(65536 p), else 0 (whatever x holds there); 0 <= p and
+ * t < 65536.  The mask is never stored: the backward pass is the same call on the gradient.  `out` may be `x` itself. */
+int gymhip_dropout(const void* x, int type, int64_t rows, int64_t width, int64_t stride, double p, const gymhip_random_keys* keys, void* out,
+                   int64_t out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
