@@ -1,0 +1,330 @@
+// policy_rules.hip — element by element: the rules on logits with their gradient, and the gradient of an action's score.
+#include "policy_common.h"
+
+namespace gymhip {
+namespace policy {
+namespace {
+
+// A workgroup takes a tile of R rows by C columns, C = lanes * kVec * NV with `lanes` a power of two: a row of at most kBlock * kVec * NV
+// columns is one tile's row (and several of them share a workgroup), a wider one is cut into tiles along its columns.
+// Each thread keeps NV 16-byte loads in flight.
+constexpr int kNv = 4;
+
+struct Tiling {
+    int lanes_log2;      // lanes that share a row
+    int nv;              // vectors per lane, <= kNv
+    int64_t cuts;        // tiles along a row
+    int64_t tiles;       // tiles in all
+};
+
+template <typename E>
+Tiling tiling(int64_t rows, int64_t width) {
+    Tiling t;
+    t.lanes_log2 = 0;
+    while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) < width) t.lanes_log2++;
+    const int64_t step = (int64_t)E::kVec << t.lanes_log2;
+    const int64_t need = (width + step - 1) / step;
+    t.nv = (int)(need < kNv ? need : kNv);
+    t.cuts = (width + step * t.nv - 1) / (step * t.nv);
+    const int64_t per = kBlock >> t.lanes_log2;
+    t.tiles = (rows + per - 1) / per * t.cuts;
+    return t;
+}
+
+// Calls f(row state w, row b, first column v0, counts of the vector or null) for every vector of this thread in every tile of the workgroup;
+// `begin(b)` makes the row's state.
+template <typename E, bool RULES, typename Begin, typename F>
+__device__ inline void each_vector(const Rules& r, const Tiling& t, int64_t rows, int64_t width, uint32_t* counts, Begin begin, F f) {
+    const int lanes = 1 << t.lanes_log2, per = kBlock >> t.lanes_log2, cap = (E::kVec << t.lanes_log2) * t.nv;
+    const int mine = (int)threadIdx.x >> t.lanes_log2, lane = (int)threadIdx.x & (lanes - 1);
+    for (int64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
+        const int64_t band = t.cuts == 1 ? tile : tile / t.cuts;
+        const int64_t lo = t.cuts == 1 ? 0 : (tile - band * t.cuts) * cap;
+        if (RULES && r.hist) count_ids(r, band * per, per, rows, width, lo, cap, counts);
+        const int64_t b = band * per + mine;
+        if (b < rows) {
+            const auto w = begin(b);
+            f(w, b, lo + lane * E::kVec, (int64_t)lanes * E::kVec, RULES && r.hist ? counts + mine * cap + lane * E::kVec : nullptr);
+        }
+    }
+}
+
+// z = y / T.  Without a penalty or a bias x / T is one correctly rounded float division; else y is a double, divided and rounded once.
+__device__ inline float processed(const Row& w, float xf, uint32_t count, bool ok, int64_t v) {
+    if (!ok) return -INFINITY;
+    if (!count && !w.bias) return xf / w.temp;
+    return (float)(ruled(w, xf, count, true, v) / (double)w.temp);
+}
+
+// g * dz/dx
+__device__ inline float sloped(const Row& w, float g, float xf, uint32_t count, bool ok) {
+    if (!ok) return 0.f;
+    if (!count) return g / w.temp;
+    const double s = xf > 0.f ? 1.0 / (double)w.rep : (double)w.rep;
+    return (float)((double)g * s / (double)w.temp);
+}
+
+template <typename E, bool RULES>
+__global__ void __launch_bounds__(kBlock) process_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
+                                                         typename E::T* out, int64_t out_stride) {
+    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
+    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return row_of<RULES>(r, b); },
+                          [&](const Row& w, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
+        float v[kNv][E::kVec];
+#pragma unroll
+        for (int k = 0; k < kNv; k++)
+            if (k < t.nv && v0 + k * step < width) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);
+#pragma unroll
+        for (int k = 0; k < kNv; k++) {
+            const int64_t at = v0 + k * step;
+            if (k >= t.nv || at >= width) continue;
+            const uint32_t bits = RULES ? allowed_bits(w, at) : 0xFFu;
+#pragma unroll
+            for (int j = 0; j < E::kVec; j++)
+                v[k][j] = processed(w, v[k][j], c ? c[k * step + j] : 0u, bits >> j & 1, at + j < width ? at + j : 0);
+            store_cols<E>(out + b * out_stride, at, width, v[k]);
+        }
+    });
+}
+
+template <typename E, bool RULES>
+__global__ void __launch_bounds__(kBlock) process_backward_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
+                                                                  const typename E::T* g, int64_t g_stride, typename E::T* out, int64_t out_stride) {
+    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
+    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return row_of<RULES>(r, b); },
+                          [&](const Row& w, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
+        float v[kNv][E::kVec], u[kNv][E::kVec];
+#pragma unroll
+        for (int k = 0; k < kNv; k++)
+            if (k < t.nv && v0 + k * step < width) {
+                load_cols<E>(g + b * g_stride, v0 + k * step, width, u[k], 0.f);
+                if (RULES && c) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);   // only its sign, and only under a penalty
+            }
+#pragma unroll
+        for (int k = 0; k < kNv; k++) {
+            const int64_t at = v0 + k * step;
+            if (k >= t.nv || at >= width) continue;
+            const uint32_t bits = RULES ? allowed_bits(w, at) : 0xFFu;
+#pragma unroll
+            for (int j = 0; j < E::kVec; j++) u[k][j] = sloped(w, u[k][j], RULES && c ? v[k][j] : 0.f, RULES && c ? c[k * step + j] : 0u, bits >> j & 1);
+            store_cols<E>(out + b * out_stride, at, width, u[k]);
+        }
+    });
+}
+
+struct ScoreRow {
+    Row w;
+    int64_t act;
+    double base;            // max y
+    float k, ls2, gl, ge, ent, inv_temp;
+    bool empty;
+};
+
+// dx = (delta gl - p (gl + ge (log p + H))) dz/dx with p = 2^((y - max y) log2 e / T - log2 S), in float32; y - max y is taken before anything is
+// rounded, so p is as exact far from 0 as near it.
+template <typename E, bool RULES>
+__global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
+                                                                const void* actions, int act64, const float* log_prob, const float* entropy,
+                                                                const double* log_sum, const float* g_lp, const float* g_ent,
+                                                                typename E::T* out, int64_t out_stride) {
+    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
+    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) {
+        ScoreRow s;
+        s.w = row_of<RULES>(r, b);
+        s.act = act64 ? ((const int64_t*)actions)[b] : (int64_t)((const int32_t*)actions)[b];
+        s.base = log_sum[2 * b];
+        const double ls = log_sum[2 * b + 1];
+        s.empty = ls == -INFINITY;
+        s.ls2 = (float)(ls * kLog2e);
+        s.k = (float)(kLog2e / (double)s.w.temp);
+        s.gl = !g_lp || log_prob[b] == -INFINITY ? 0.f : g_lp[b];
+        s.ge = g_ent ? g_ent[b] : 0.f;
+        s.ent = entropy[b];
+        s.inv_temp = 1.f / s.w.temp;
+        return s;
+    }, [&](const ScoreRow& s, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
+        float v[kNv][E::kVec];
+#pragma unroll
+        for (int k = 0; k < kNv; k++)
+            if (k < t.nv && v0 + k * step < width) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);
+#pragma unroll
+        for (int k = 0; k < kNv; k++) {
+            const int64_t at = v0 + k * step;
+            if (k >= t.nv || at >= width) continue;
+            const uint32_t bits = s.empty ? 0u : RULES ? allowed_bits(s.w, at) : 0xFFu;
+            const int64_t hot = s.act - at;
+#pragma unroll
+            for (int j = 0; j < E::kVec; j++) {
+                const uint32_t n = RULES && c ? c[k * step + j] : 0u;
+                const float xf = v[k][j];
+                float d;
+                if (!RULES) d = xf - (float)s.base;   // the greatest logit: exact in float
+                else d = (float)(ruled(s.w, xf, n, true, at + j < width ? at + j : 0) - s.base);
+                const float lp2 = d * s.k - s.ls2;
+                const float p = __builtin_amdgcn_exp2f(lp2);
+                const float lp = (lp2 < -200.f ? -200.f : lp2) * (float)kLn2;   // p is 0 there; keeps 0 * inf out
+                float g = (hot == j ? s.gl : 0.f) - p * (s.gl + s.ge * (lp + s.ent));
+                g *= s.inv_temp;
+                if (RULES && n) g *= xf > 0.f ? 1.f / s.w.rep : s.w.rep;
+                v[k][j] = bits >> j & 1 ? g : 0.f;
+            }
+            store_cols<E>(out + b * out_stride, at, width, v[k]);
+        }
+    });
+}
+
+int64_t element_size(int type) { return type == GYMHIP_TYPE_F32 ? 4 : 2; }
+
+}  // namespace
+
+// ---- host side: the checks every policy entry point makes ----------------------------------------------------------------------------------
+int check_matrix(const char* what, const void* data, int type, int64_t rows, int64_t width, int64_t stride) {
+    if (type != GYMHIP_TYPE_F32 && type != GYMHIP_TYPE_F16 && type != GYMHIP_TYPE_BF16) return fail(GYMHIP_EINVAL, "type must be GYMHIP_TYPE_F32, _F16 or _BF16");
+    if (rows < 0 || rows > (1ll << 40) || width < 0 || width > GYMHIP_POLICY_MAX_WIDTH) return fail(GYMHIP_EINVAL, "rows or width out of range (width <= 2^24)");
+    if (rows && width && !data) return fail(GYMHIP_EINVAL, "%s is null", what);
+    if (stride < 0 || (rows > 1 && stride > 0x7fffffffffffffffll / 8 / rows)) return fail(GYMHIP_EINVAL, "%s: stride out of range", what);
+    if ((uintptr_t)data % (uintptr_t)element_size(type)) return fail(GYMHIP_EINVAL, "%s is not aligned to its type", what);
+    return GYMHIP_OK;
+}
+
+// An output's rows must not share elements, and it may coincide with an input only element for element.
+int check_output(const char* what, const void* out, int type, int64_t rows, int64_t width, int64_t stride, const void* in, int64_t in_stride) {
+    if (int rc = check_matrix(what, out, type, rows, width, stride)) return rc;
+    if (rows > 1 && stride < width) return fail(GYMHIP_EINVAL, "%s: rows overlap (stride < width)", what);
+    if (!in || !rows || !width || (in == out && (in_stride == stride || rows == 1))) return GYMHIP_OK;
+    const uintptr_t e = (uintptr_t)element_size(type);
+    const uintptr_t a = (uintptr_t)out, a1 = a + ((uintptr_t)(rows - 1) * (uintptr_t)stride + (uintptr_t)width) * e;
+    const uintptr_t c = (uintptr_t)in, c1 = c + ((uintptr_t)(rows - 1) * (uintptr_t)in_stride + (uintptr_t)width) * e;
+    if (a < c1 && c < a1) return fail(GYMHIP_EINVAL, "%s overlaps an input", what);
+    return GYMHIP_OK;
+}
+
+int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules* out) {
+    *out = Rules{};
+    out->rep = out->temp = 1.f;
+    if (!r) return GYMHIP_OK;
+    if (r->struct_size != (int32_t)sizeof(gymhip_logit_rules)) return fail(GYMHIP_EINVAL, "bad gymhip_logit_rules.struct_size");
+    if (r->mask) {
+        if (r->mask_lines < 1) return fail(GYMHIP_EINVAL, "mask_lines must be positive");
+        if (!r->mask_rows && r->mask_lines != 1 && r->mask_lines != rows) return fail(GYMHIP_EINVAL, "without mask_rows, mask_lines must be 1 or rows");
+        if (r->mask_stride < 0 || (r->mask_lines > 1 && r->mask_stride < (width + 31) / 32)) return fail(GYMHIP_EINVAL, "mask lines are shorter than ceil(width / 32) words");
+    } else if (r->mask_rows) {
+        return fail(GYMHIP_EINVAL, "mask_rows without a mask");
+    }
+    if (r->bias && r->bias_stride < 0) return fail(GYMHIP_EINVAL, "bias_stride must not be negative");
+    if (r->history) {
+        if (r->history_dtype != GYMHIP_ACT_I32 && r->history_dtype != GYMHIP_ACT_I64) return fail(GYMHIP_EINVAL, "history_dtype must be GYMHIP_ACT_I32 or _I64");
+        if (r->history_len && r->history_len_dtype != GYMHIP_ACT_I32 && r->history_len_dtype != GYMHIP_ACT_I64)
+            return fail(GYMHIP_EINVAL, "history_len_dtype must be GYMHIP_ACT_I32 or _I64");
+        if (r->history_cols < 0 || r->history_cols > 0x7fffffff || r->history_stride < 0) return fail(GYMHIP_EINVAL, "history size out of range");
+    } else if (r->history_len) {
+        return fail(GYMHIP_EINVAL, "history_len without a history");
+    }
+    if (!r->repetition_rows && !(r->repetition > 0.f && std::isfinite(r->repetition))) return fail(GYMHIP_EINVAL, "repetition must be positive and finite");
+    if (!r->temperature_rows && !(r->temperature >= 0.f && std::isfinite(r->temperature))) return fail(GYMHIP_EINVAL, "temperature must be finite and not negative");
+    if ((!r->presence_rows && !std::isfinite(r->presence)) || (!r->frequency_rows && !std::isfinite(r->frequency)))
+        return fail(GYMHIP_EINVAL, "presence and frequency must be finite");
+    out->mask = r->mask; out->mask_stride = r->mask_stride; out->mask_lines = r->mask_lines; out->mask_rows = r->mask_rows;
+    out->bias = r->bias; out->bias_stride = r->bias_stride;
+    if (r->history && r->history_cols > 0) {
+        out->hist = r->history; out->hist_stride = r->history_stride; out->hist_cols = (uint32_t)r->history_cols; out->hist_len = r->history_len;
+        out->hist64 = r->history_dtype == GYMHIP_ACT_I64; out->len64 = r->history_len_dtype == GYMHIP_ACT_I64;
+    }
+    out->rep_rows = r->repetition_rows; out->pres_rows = r->presence_rows; out->freq_rows = r->frequency_rows; out->temp_rows = r->temperature_rows;
+    out->rep = r->repetition; out->pres = r->presence; out->freq = r->frequency; out->temp = r->temperature;
+    return GYMHIP_OK;
+}
+
+int check_keys(const gymhip_random_keys* k, Keys* out) {
+    if (!k || k->struct_size != (int32_t)sizeof(gymhip_random_keys)) return fail(GYMHIP_EINVAL, "keys: null, or bad gymhip_random_keys.struct_size");
+    out->seed = k->seed; out->row = k->row; out->step = k->step; out->rows = k->rows; out->steps = k->steps; out->steps_per_row = k->steps_per_row != 0;
+    return GYMHIP_OK;
+}
+
+int check_actions(const void* actions, int dtype, int64_t rows) {
+    if (rows && !actions) return fail(GYMHIP_EINVAL, "actions is null");
+    if (dtype != GYMHIP_ACT_I32 && dtype != GYMHIP_ACT_I64) return fail(GYMHIP_EINVAL, "action_dtype must be GYMHIP_ACT_I32 or GYMHIP_ACT_I64");
+    return GYMHIP_OK;
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t needed) {
+    if (!needed) return GYMHIP_OK;
+    if (!workspace || bytes < needed) return fail(GYMHIP_EINVAL, "workspace: %zu bytes needed, %zu given", needed, workspace ? bytes : (size_t)0);
+    if ((uintptr_t)workspace % 16) return fail(GYMHIP_EINVAL, "workspace is not 16-byte aligned");
+    return GYMHIP_OK;
+}
+
+int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GYMHIP_OK : fail(GYMHIP_EHIP, "launch failed: %s", hipGetErrorString(e));
+}
+
+}  // namespace policy
+}  // namespace gymhip
+
+using namespace gymhip;
+using namespace gymhip::policy;
+
+extern "C" {
+
+int gymhip_process_logits(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules, void* out,
+                          int64_t out_stride, void* stream) {
+    Rules r;
+    if (int rc = check_matrix("logits", logits, type, rows, width, stride)) return rc;
+    if (int rc = check_output("out", out, type, rows, width, out_stride, logits, stride)) return rc;
+    if (int rc = check_rules(rules, rows, width, &r)) return rc;
+    if (!rows || !width) return GYMHIP_OK;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        using T = typename E::T;
+        with_bool(!r.plain(), [&](auto ruled_) {
+            const Tiling t = tiling<E>(rows, width);
+            hipLaunchKernelGGL((process_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream, (const T*)logits, rows,
+                               width, stride, r, t, (T*)out, out_stride);
+        });
+    });
+}
+
+int gymhip_process_logits_backward(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                                   const void* grad_out, int64_t grad_out_stride, void* grad_in, int64_t grad_in_stride, void* stream) {
+    Rules r;
+    if (int rc = check_matrix("logits", logits, type, rows, width, stride)) return rc;
+    if (int rc = check_matrix("grad_out", grad_out, type, rows, width, grad_out_stride)) return rc;
+    if (int rc = check_output("grad_in", grad_in, type, rows, width, grad_in_stride, logits, stride)) return rc;
+    if (int rc = check_output("grad_in", grad_in, type, rows, width, grad_in_stride, grad_out, grad_out_stride)) return rc;
+    if (int rc = check_rules(rules, rows, width, &r)) return rc;
+    if (!rows || !width) return GYMHIP_OK;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        using T = typename E::T;
+        with_bool(!r.plain(), [&](auto ruled_) {
+            const Tiling t = tiling<E>(rows, width);
+            hipLaunchKernelGGL((process_backward_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream,
+                               (const T*)logits, rows, width, stride, r, t, (const T*)grad_out, grad_out_stride, (T*)grad_in, grad_in_stride);
+        });
+    });
+}
+
+int gymhip_action_log_prob_backward(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
+                                    const void* actions, int action_dtype, const float* log_prob, const float* entropy, const double* log_sum,
+                                    const float* grad_log_prob, const float* grad_entropy, void* grad_in, int64_t grad_in_stride, void* stream) {
+    Rules r;
+    if (int rc = check_matrix("logits", logits, type, rows, width, stride)) return rc;
+    if (int rc = check_output("grad_in", grad_in, type, rows, width, grad_in_stride, logits, stride)) return rc;
+    if (int rc = check_rules(rules, rows, width, &r)) return rc;
+    if (int rc = check_actions(actions, action_dtype, rows)) return rc;
+    if (rows && (!log_prob || !entropy || !log_sum)) return fail(GYMHIP_EINVAL, "log_prob, entropy or log_sum is null");
+    if (!rows || !width) return GYMHIP_OK;
+    return with_type(type, [&](auto e) {
+        using E = decltype(e);
+        using T = typename E::T;
+        with_bool(!r.plain(), [&](auto ruled_) {
+            const Tiling t = tiling<E>(rows, width);
+            hipLaunchKernelGGL((score_backward_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream,
+                               (const T*)logits, rows, width, stride, r, t, actions, (int)(action_dtype == GYMHIP_ACT_I64), log_prob, entropy, log_sum,
+                               grad_log_prob, grad_entropy, (T*)grad_in, grad_in_stride);
+        });
+    });
+}
+
+}  // extern "C"
