@@ -17,18 +17,18 @@ constexpr int kBlock = 256;
 constexpr int kWave = 64;
 
 // ---- element types: kVec elements are 16 bytes; loads widen to float, stores round once, to nearest even -------------------------------
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 struct F32 {
     using T = float;
     static constexpr int kVec = 4;
-    __device__ static float widen(uint32_t word, int) { return __uint_as_float(word); }
+    static constexpr uint32_t kNone = 0xFF800000u;   // -inf
+    __device__ static float widen(const uint32_t* w, int j) { return __uint_as_float(w[j]); }
     __device__ static uint32_t narrow(const float* v) { return __float_as_uint(v[0]); }
 };
 struct F16 {
     using T = _Float16;
     static constexpr int kVec = 8;
-    __device__ static float widen(uint32_t word, int half) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(half ? word >> 16 : word)); }
+    static constexpr uint32_t kNone = 0xFC00FC00u;
+    __device__ static float widen(const uint32_t* w, int j) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2])); }
     __device__ static uint32_t narrow(const float* v) {
         return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[0]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16;
     }
@@ -36,43 +36,63 @@ struct F16 {
 struct BF16 {
     using T = __bf16;
     static constexpr int kVec = 8;
-    __device__ static float widen(uint32_t word, int half) { return __uint_as_float(half ? word & 0xFFFF0000u : word << 16); }
+    static constexpr uint32_t kNone = 0xFF80FF80u;
+    __device__ static float widen(const uint32_t* w, int j) { return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16); }
     __device__ static uint32_t narrow(const float* v) {
         return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[0]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[1]) << 16;
     }
 };
 
-// kVec columns from v0 on, as floats.  The address has the element's alignment only (odd strides, odd starts); the hardware takes 16-byte
-// accesses at any such address, so a row needs no aligned middle of its own.  Columns past the row's end read as `absent`, unread.
-template <typename E>
-__device__ inline void load_cols(const typename E::T* row, int64_t v0, int64_t width, float* out, float absent) {
+// C adjacent elements of a row, as they lie in memory: C * sizeof(T) is 4, 8 or 16 bytes.  The address has the element's alignment only (odd
+// strides, odd starts); the hardware takes 16-byte accesses at any such address, so a row needs no aligned middle of its own.
+template <typename E, int C>
+struct Raw {
     using T = typename E::T;
-    if (v0 + E::kVec <= width) {
-        struct __attribute__((packed, aligned(sizeof(T)))) U { u32x4 w; };
-        const u32x4 w = ((const U*)(row + v0))->w;
-#pragma unroll
-        for (int j = 0; j < E::kVec; j++) out[j] = E::kVec == 4 ? E::widen(w[j], 0) : E::widen(w[j / 2], j & 1);
-    } else {
-#pragma unroll
-        for (int j = 0; j < E::kVec; j++) out[j] = v0 + j < width ? (float)row[v0 + j] : absent;
-    }
-}
+    static constexpr int kWords = C * (int)sizeof(T) / 4;
+    uint32_t w[kWords];
+    struct __attribute__((packed, aligned(sizeof(T)))) Packed { uint32_t w[kWords]; };
 
-template <typename E>
-__device__ inline void store_cols(typename E::T* row, int64_t v0, int64_t width, const float* v) {
-    using T = typename E::T;
-    if (v0 + E::kVec <= width) {
-        struct __attribute__((packed, aligned(sizeof(T)))) U { u32x4 w; };
-        u32x4 w;
+    // Columns from v0 on; those behind the row's end are -inf, and not read.
+    __device__ void load(const T* row, int64_t v0, int64_t width) {
+        if (v0 + C <= width) {
+            const Packed p = *(const Packed*)(row + v0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = E::narrow(v + (E::kVec == 4 ? j : 2 * j));
-        ((U*)(row + v0))->w = w;
-    } else {
+            for (int i = 0; i < kWords; i++) w[i] = p.w[i];
+        } else {
 #pragma unroll
-        for (int j = 0; j < E::kVec; j++)
-            if (v0 + j < width) row[v0 + j] = (T)v[j];
+            for (int i = 0; i < kWords; i++) w[i] = E::kNone;
+#pragma unroll
+            for (int j = 0; j < C; j++)
+                if (v0 + j < width) {
+                    if (sizeof(T) == 4) w[j] = ((const uint32_t*)row)[v0 + j];
+                    else {
+                        const uint32_t e = ((const uint16_t*)row)[v0 + j];
+                        w[j / 2] = j & 1 ? (w[j / 2] & 0xFFFFu) | e << 16 : (w[j / 2] & 0xFFFF0000u) | e;
+                    }
+                }
+        }
     }
-}
+    __device__ float get(int j) const { return E::widen(w, j); }
+    __device__ void set(const float* v) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) w[i] = E::narrow(v + i * C / kWords);
+    }
+    __device__ void store(T* row, int64_t v0, int64_t width) const {
+        if (v0 + C <= width) {
+            Packed p;
+#pragma unroll
+            for (int i = 0; i < kWords; i++) p.w[i] = w[i];
+            *(Packed*)(row + v0) = p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; j++)
+                if (v0 + j < width) {
+                    if (sizeof(T) == 4) ((uint32_t*)row)[v0 + j] = w[j];
+                    else ((uint16_t*)row)[v0 + j] = (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+                }
+        }
+    }
+};
 
 // ---- random numbers ------------------------------------------------------------------------------------------------------------------
 struct Keys {
@@ -133,7 +153,7 @@ struct Rules {
 struct Row {
     const uint32_t* mask;   // its line, or null where everything is allowed
     const float* bias;
-    float rep, pres, freq, temp;
+    double rep, inv_rep, pres, freq, temp;
     bool greedy, nothing;   // nothing: its line lies behind the mask's last one
 };
 
@@ -142,11 +162,12 @@ __device__ inline Row row_of(const Rules& r, int64_t b) {
     Row w;
     const float t = r.temp_rows ? r.temp_rows[b] : r.temp;
     w.greedy = !(t > 0.f);
-    w.temp = w.greedy ? 1.f : t;
+    w.temp = w.greedy ? 1.0 : (double)t;
     w.mask = nullptr;
     w.bias = nullptr;
     w.nothing = false;
-    w.rep = w.pres = w.freq = 0.f;
+    w.rep = w.inv_rep = 1.0;
+    w.pres = w.freq = 0.0;
     if (RULES) {
         if (r.mask) {
             const int64_t line = r.mask_rows ? r.mask_rows[b] : (r.mask_lines == 1 ? 0 : b);
@@ -156,6 +177,7 @@ __device__ inline Row row_of(const Rules& r, int64_t b) {
         if (r.bias) w.bias = r.bias + b * r.bias_stride;
         if (r.hist) {
             w.rep = r.rep_rows ? r.rep_rows[b] : r.rep;
+            w.inv_rep = 1.0 / w.rep;
             w.pres = r.pres_rows ? r.pres_rows[b] : r.pres;
             w.freq = r.freq_rows ? r.freq_rows[b] : r.freq;
         }
@@ -163,61 +185,139 @@ __device__ inline Row row_of(const Rules& r, int64_t b) {
     return w;
 }
 
-// The mask's bits of kVec (4 or 8) columns from v0 on, v0 a multiple of kVec and < width.
+// x / d as IEEE rounds it, with inv = 1 / d rounded: the quotient's remainder is exact in one fma and corrects it (Markstein's theorem; x and d
+// are far from a double's range, being floats or sums of a few).  Infinities and NaN, whose remainder is NaN, keep the first quotient.
+__device__ inline double divided(double x, double d, double inv) {
+    const double q = x * inv;
+    const double c = __builtin_fma(__builtin_fma(-q, d, x), inv, q);
+    return fabs(q) < INFINITY ? c : q;
+}
+
+// The mask's bits of C (at most 8) columns from v0 on, v0 a multiple of C and < width.
 __device__ inline uint32_t allowed_bits(const Row& w, int64_t v0) {
     if (w.nothing) return 0u;
     return w.mask ? w.mask[v0 >> 5] >> (v0 & 31) : 0xFFu;
 }
 
-// y: the logit after penalties and bias, before the temperature.  In double: what is compared and summed must be the formula's value even
-// where a bias or a penalty cancels most of the logit.
-__device__ inline double penalised(const Row& w, float xf, uint32_t count) {
-    double x = xf;
-    if (count) {
-        x = x > 0 ? x / (double)w.rep : x * (double)w.rep;
-        x = x - (double)w.freq * (double)count - (double)w.pres;
-    }
-    return x;
+// x under the penalties of a count > 0.
+__device__ inline double penalised(const Row& w, double x, uint32_t count) {
+    const double y = x > 0 ? divided(x, w.rep, w.inv_rep) : x * w.rep;
+    return y - w.freq * (double)count - w.pres;
 }
+// y of one column.
 __device__ inline double ruled(const Row& w, float xf, uint32_t count, bool ok, int64_t v) {
-    if (!ok) return -INFINITY;
-    const double x = penalised(w, xf, count);
-    return w.bias ? x + (double)w.bias[v] : x;
+    double y = xf;
+    if (count) y = penalised(w, y, count);
+    if (w.bias) y += (double)w.bias[v];
+    return ok ? y : -INFINITY;
 }
 
-// How often each id of columns [lo, lo + cap) occurs in the histories of rows [b0, b0 + n): counts[row - b0][id - lo], by the whole workgroup.
-// The rows' ids are read as one run of n * hist_cols places (adjacent rows' ids are adjacent in memory); integer LDS atomics, so their
-// order is free.  Every thread of the workgroup comes here; counts may be read after it returns.
+// y of C columns from v0 on: the logits after penalties and bias, before the temperature; -inf where the mask does not allow.  In double (which
+// runs at the rate of float here): what is compared and summed must be the formula's value even where a bias or a penalty cancels most of
+// the logit.  Straight-line code: a wave passes over the penalties only where none of its lanes has a count.
+// `counts`: the columns' counts, or null for the whole workgroup.
+template <typename E, int C>
+__device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, int64_t v0, int64_t width, const uint32_t* counts, double* y) {
+    const uint32_t bits = allowed_bits(w, v0);
+#pragma unroll
+    for (int j = 0; j < C; j++) y[j] = (double)raw.get(j);
+    if (counts) {
+        uint32_t c[C], any = 0;
+#pragma unroll
+        for (int j = 0; j < C; j++) any |= c[j] = counts[j];
+        if (__any(any)) {
+#pragma unroll
+            for (int j = 0; j < C; j++) {
+                const double p = penalised(w, y[j], c[j]);
+                y[j] = c[j] ? p : y[j];
+            }
+        }
+    }
+    if (w.bias) {
+        float f[C];
+        if (v0 + C <= width) {
+            struct __attribute__((packed, aligned(4))) Packed { float f[C]; };
+            const Packed p = *(const Packed*)(w.bias + v0);
+#pragma unroll
+            for (int j = 0; j < C; j++) f[j] = p.f[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; j++) f[j] = v0 + j < width ? w.bias[v0 + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < C; j++) y[j] += (double)f[j];
+    }
+#pragma unroll
+    for (int j = 0; j < C; j++) y[j] = bits >> j & 1 ? y[j] : -INFINITY;
+}
+
+// How often each id of columns [lo, lo + cap) occurs in the histories of rows [b0, b0 + n): counts[(row - b0) * cap + id - lo], by the whole
+// workgroup.  Integer LDS atomics, so their order is free.  Every thread of the workgroup comes here; counts may be read after it returns.
+// cap * n is a multiple of 4, counts 16-byte aligned.
+template <typename Id>
+__device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_t span, int first, int step, uint32_t* counts) {
+    struct __attribute__((packed, aligned(sizeof(Id)))) Four { Id v[4]; };
+    for (int64_t i = (int64_t)first * 4; i < len; i += (int64_t)step * 4) {
+        if (i + 4 <= len) {
+            const Four f = *(const Four*)(ids + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint64_t at = (uint64_t)((int64_t)f.v[j] - lo);
+                if (at < span) atomicAdd(&counts[at], 1u);
+            }
+        } else {
+            for (int64_t j = i; j < len; j++) {
+                const uint64_t at = (uint64_t)((int64_t)ids[j] - lo);
+                if (at < span) atomicAdd(&counts[at], 1u);
+            }
+        }
+    }
+}
 __device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows, int64_t width, int64_t lo, int cap, uint32_t* counts) {
     __syncthreads();
-    for (int i = threadIdx.x; i < n * cap; i += kBlock) counts[i] = 0;
+    for (int i = threadIdx.x; i < n * cap / 4; i += kBlock) ((uint4*)counts)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const uint32_t cols = r.hist_cols;
-    const int64_t hi = lo + cap < width ? lo + cap : width;
-    for (uint64_t i = threadIdx.x; i < (uint64_t)n * cols; i += kBlock) {
-        uint32_t q = 0, c = (uint32_t)i;
-        if (n > 1) {
-            if ((uint64_t)n * cols <= 0xFFFFFFFFull) { q = (uint32_t)i / cols; c = (uint32_t)i - q * cols; }
-            else { q = (uint32_t)(i / cols); c = (uint32_t)(i - (uint64_t)q * cols); }
-        }
-        const int64_t b = b0 + q;
-        if (b >= rows) break;
+    const uint32_t span = (uint32_t)(lo + cap < width ? cap : width - lo);
+    const int each = kBlock / n, mine = (int)threadIdx.x / each;   // n is a power of two: `each` adjacent threads take a row
+    const int64_t b = b0 + mine;
+    if (b < rows) {
+        int64_t len = r.hist_cols;
         if (r.hist_len) {
-            const int64_t len = r.len64 ? ((const int64_t*)r.hist_len)[b] : (int64_t)((const int32_t*)r.hist_len)[b];
-            if ((int64_t)c >= len) continue;
+            const int64_t have = r.len64 ? ((const int64_t*)r.hist_len)[b] : (int64_t)((const int32_t*)r.hist_len)[b];
+            len = have < len ? have : len;
         }
-        const int64_t at = b * r.hist_stride + c;
-        const int64_t id = r.hist64 ? ((const int64_t*)r.hist)[at] : (int64_t)((const int32_t*)r.hist)[at];
-        if (id >= lo && id < hi) atomicAdd(&counts[q * cap + (int)(id - lo)], 1u);
+        const int first = (int)threadIdx.x & (each - 1);
+        if (r.hist64) count_row((const int64_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, counts + mine * cap);
+        else count_row((const int32_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, counts + mine * cap);
     }
     __syncthreads();
 }
 
-// ---- reductions over G lanes: G <= 64 adjacent lanes of a wave by exchange, G = kBlock through LDS as well ---------------------------------
+// ---- reductions over G lanes: G <= 64 adjacent lanes of a wave by lane permutations in the vector unit, G = kBlock through LDS as well --------
+template <int CTRL, int ROWS = 0xF>
+__device__ inline uint32_t permuted(uint32_t v, uint32_t else_) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)else_, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS = 0xF, typename V>
+__device__ inline V permuted_value(V v, V else_) {
+    static_assert(sizeof(V) == 4 || sizeof(V) == 8, "");
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, permuted<CTRL, ROWS>(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, else_)));
+    } else {
+        const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, else_);
+        const uint64_t lo = permuted<CTRL, ROWS>((uint32_t)a, (uint32_t)b), hi = permuted<CTRL, ROWS>((uint32_t)(a >> 32), (uint32_t)(b >> 32));
+        return __builtin_bit_cast(V, hi << 32 | lo);
+    }
+}
+
 template <int G, typename V, typename Op>
 __device__ inline V group_reduce(V v, Op op, V* lds) {
-#pragma unroll
-    for (int s = 1; s < (G < kWave ? G : kWave); s <<= 1) v = op(v, __shfl_xor(v, s));
+    if (G >= 2) v = op(v, permuted_value<0xB1>(v, v));    // lane ^ 1
+    if (G >= 4) v = op(v, permuted_value<0x4E>(v, v));    // lane ^ 2
+    if (G >= 8) v = op(v, permuted_value<0x141>(v, v));   // 7 - lane: the other four, which by now hold one value
+    if (G >= 16) v = op(v, permuted_value<0x140>(v, v));  // 15 - lane
+    if (G >= 32) v = op(v, __shfl_xor(v, 16));
+    if (G >= 64) v = op(v, __shfl_xor(v, 32));
     if (G > kWave) {
         __syncthreads();
         if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
@@ -229,76 +329,50 @@ __device__ inline V group_reduce(V v, Op op, V* lds) {
     return v;
 }
 
+// Sums over lanes 0 .. lane of each group of W <= 64 lanes.
+template <int W>
+__device__ inline double running_sum(double v, int lane) {
+    if (W >= 2) { const double o = permuted_value<0x111>(v, 0.0); v += lane >= 1 ? o : 0.0; }
+    if (W >= 4) { const double o = permuted_value<0x112>(v, 0.0); v += lane >= 2 ? o : 0.0; }
+    if (W >= 8) { const double o = permuted_value<0x114>(v, 0.0); v += lane >= 4 ? o : 0.0; }
+    if (W >= 16) { const double o = permuted_value<0x118>(v, 0.0); v += lane >= 8 ? o : 0.0; }
+    if (W >= 32) v += permuted_value<0x142, 0xA>(v, 0.0);   // the last lane of a row of 16 to the next row
+    if (W >= 64) v += permuted_value<0x143, 0xC>(v, 0.0);   // lane 31 to the upper half
+    return v;
+}
+
 template <typename V> struct Max { __device__ V operator()(V a, V b) const { return a > b ? a : b; } };   // of values without NaN
 template <typename V> struct Min { __device__ V operator()(V a, V b) const { return a < b ? a : b; } };
 template <typename V> struct Sum { __device__ V operator()(V a, V b) const { return a + b; } };
 
-// 2^t in double to 2e-14 of its value, for -1000 <= t <= 1000: t = n + f, |f| <= 1/2, and a polynomial of degree 9 through the Chebyshev nodes
-// for 2^f.  18 instructions, all at the double (= single) rate.
+// 2^t in double to 4e-16 of its value, for -1000 <= t <= 1000: t = n + f, |f| <= 1/2, and a polynomial of degree 10 through the Chebyshev nodes
+// for 2^f.  16 instructions, all at the double (= float) rate.
 __device__ inline double exp2_double(double t) {
     const double shifted = t + 0x1.8p52;                                     // n in the low word
     const double f = t - (shifted - 0x1.8p52);
-    double p = 0x1.b6571de2f2351p-24;
-    p = __builtin_fma(p, f, 0x1.63ef969a64d3cp-20);
-    p = __builtin_fma(p, f, 0x1.ffcb76789860fp-17);
-    p = __builtin_fma(p, f, 0x1.43088e257f341p-13);
-    p = __builtin_fma(p, f, 0x1.5d87fe908f88ap-10);
-    p = __builtin_fma(p, f, 0x1.3b2ab72b175eep-7);
-    p = __builtin_fma(p, f, 0x1.c6b08d7044119p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbdff8149f2p-3);
-    p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
-    p = __builtin_fma(p, f, 0x1.000000000003dp+0);
+    double p = 0x1.e6063f7217bc6p-28;
+    p = __builtin_fma(p, f, 0x1.b675bca4eeebbp-24);
+    p = __builtin_fma(p, f, 0x1.62bfd47773353p-20);
+    p = __builtin_fma(p, f, 0x1.ffcb54062e698p-17);
+    p = __builtin_fma(p, f, 0x1.430913096fd9fp-13);
+    p = __builtin_fma(p, f, 0x1.5d87fe9d7a584p-10);
+    p = __builtin_fma(p, f, 0x1.3b2ab6fba1ddap-7);
+    p = __builtin_fma(p, f, 0x1.c6b08d703ce49p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
+    p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
+    p = __builtin_fma(p, f, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
+}
+// log2 s for 1 <= s < 2^100: the float logarithm l, and s 2^-l = 1 + e with |e| < 1e-6, whose logarithm is three terms of its series.
+__device__ inline double log2_double(double s) {
+    const double l = (double)__builtin_amdgcn_logf((float)s);
+    const double e = __builtin_fma(s, exp2_double(-l), -1.0);
+    return __builtin_fma(__builtin_fma(__builtin_fma(e, 1.0 / 3.0, -0.5), e, 1.0) * e, 1.4426950408889634074, l);
 }
 // Below 2^-1000 a weight counts as none.
 constexpr double kLeast = -1000.0;
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
-
-// One thread's share of a row's tile: NV vectors of kVec columns, `step` columns apart, as y (see ruled).  Y is double under rules; float
-// where y is the logit itself.  Absent columns are -inf.  `bad` is set by a NaN.
-template <typename E, bool RULES, int NV>
-struct Tile {
-    using Y = typename std::conditional<RULES, double, float>::type;
-    Y y[NV][E::kVec];
-
-    __device__ void load(const Row& w, const typename E::T* x, int64_t v0, int64_t step, int64_t width, const uint32_t* counts, bool* bad) {
-        float f[NV][E::kVec];
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            if (NV == 1 || v0 + k * step < width) load_cols<E>(x, v0 + k * step, width, f[k], -INFINITY);
-            else
-#pragma unroll
-                for (int j = 0; j < E::kVec; j++) f[k][j] = -INFINITY;
-        }
-        bool nan = false;
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int64_t at = v0 + k * step;
-            const uint32_t bits = !RULES || at >= width ? 0xFFu : allowed_bits(w, at);
-#pragma unroll
-            for (int j = 0; j < E::kVec; j++) {
-                if (RULES) {
-                    const bool here = at + j < width;
-                    y[k][j] = ruled(w, f[k][j], here && counts ? counts[k * step + j] : 0u, bits >> j & 1, here ? at + j : 0);
-                    if (!here) y[k][j] = -INFINITY;
-                } else {
-                    y[k][j] = f[k][j];
-                }
-                nan = nan || y[k][j] != y[k][j];
-            }
-        }
-        *bad = nan;
-    }
-    __device__ Y max() const {
-        Y m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int j = 0; j < E::kVec; j++) m = y[k][j] > m ? y[k][j] : m;
-        return m;
-    }
-};
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------
 int check_matrix(const char* what, const void* data, int type, int64_t rows, int64_t width, int64_t stride);

@@ -16,16 +16,25 @@ __global__ void __launch_bounds__(kBlock) dropout_kernel(const typename E::T* x,
         const int64_t b = n >> 32 ? i / blocks : (int64_t)((uint32_t)i / (uint32_t)blocks), q = i - b * blocks;
         const uint4 w4 = row_words(keys, b, (uint32_t)q);
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        float v[8];
+        constexpr int N = 8 / E::kVec;
+        Raw<E, E::kVec> raw[N];
 #pragma unroll
-        for (int h = 0; h < 8; h += E::kVec) if (q * 8 + h < width) load_cols<E>(x + b * stride, q * 8 + h, width, v + h, 0.f);
+        for (int h = 0; h < N; h++)
+            if (q * 8 + h * E::kVec < width) raw[h].load(x + b * stride, q * 8 + h * E::kVec, width);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t bits = j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-            v[j] = bits >= limit ? v[j] * scale : 0.f;
+        for (int h = 0; h < N; h++) {
+            const int64_t at = q * 8 + h * E::kVec;
+            if (at >= width) continue;
+            float v[E::kVec];
+#pragma unroll
+            for (int j = 0; j < E::kVec; j++) {
+                const int lane = h * E::kVec + j;
+                const uint32_t bits = lane & 1 ? w[lane >> 1] >> 16 : w[lane >> 1] & 0xFFFFu;
+                v[j] = bits >= limit ? raw[h].get(j) * scale : 0.f;
+            }
+            raw[h].set(v);
+            raw[h].store(out + b * out_stride, at, width);
         }
-#pragma unroll
-        for (int h = 0; h < 8; h += E::kVec) if (q * 8 + h < width) store_cols<E>(out + b * out_stride, q * 8 + h, width, v + h);
     }
 }
 

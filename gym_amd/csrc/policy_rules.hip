@@ -31,10 +31,10 @@ Tiling tiling(int64_t rows, int64_t width) {
     return t;
 }
 
-// Calls f(row state w, row b, first column v0, counts of the vector or null) for every vector of this thread in every tile of the workgroup;
+// Calls f(row state, row b, first column v0, columns from one of the lane's vectors to its next, counts at v0 or null) once per tile;
 // `begin(b)` makes the row's state.
 template <typename E, bool RULES, typename Begin, typename F>
-__device__ inline void each_vector(const Rules& r, const Tiling& t, int64_t rows, int64_t width, uint32_t* counts, Begin begin, F f) {
+__device__ inline void each_tile(const Rules& r, const Tiling& t, int64_t rows, int64_t width, uint32_t* counts, Begin begin, F f) {
     const int lanes = 1 << t.lanes_log2, per = kBlock >> t.lanes_log2, cap = (E::kVec << t.lanes_log2) * t.nv;
     const int mine = (int)threadIdx.x >> t.lanes_log2, lane = (int)threadIdx.x & (lanes - 1);
     for (int64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
@@ -42,72 +42,103 @@ __device__ inline void each_vector(const Rules& r, const Tiling& t, int64_t rows
         const int64_t lo = t.cuts == 1 ? 0 : (tile - band * t.cuts) * cap;
         if (RULES && r.hist) count_ids(r, band * per, per, rows, width, lo, cap, counts);
         const int64_t b = band * per + mine;
-        if (b < rows) {
-            const auto w = begin(b);
-            f(w, b, lo + lane * E::kVec, (int64_t)lanes * E::kVec, RULES && r.hist ? counts + mine * cap + lane * E::kVec : nullptr);
-        }
+        if (b < rows) f(begin(b), b, lo + lane * E::kVec, lanes * E::kVec, RULES && r.hist ? counts + mine * cap + lane * E::kVec : nullptr);
     }
 }
 
-// z = y / T.  Without a penalty or a bias x / T is one correctly rounded float division; else y is a double, divided and rounded once.
-__device__ inline float processed(const Row& w, float xf, uint32_t count, bool ok, int64_t v) {
-    if (!ok) return -INFINITY;
-    if (!count && !w.bias) return xf / w.temp;
-    return (float)(ruled(w, xf, count, true, v) / (double)w.temp);
+// x / d of floats as IEEE rounds it.  inv = 1 / d, or 0 where d is not between 2^-20 and 2^20: then, and where the quotient is not between 2^-60 and
+// 2^100, the remainder may not be exact (see the double's `divided`) and the division itself is made.
+__device__ inline float dividedf(float x, float d, float inv) {
+    const float q = x * inv, a = fabsf(q);
+    if (a > 0x1p-60f && a < 0x1p100f) return __builtin_fmaf(__builtin_fmaf(-q, d, x), inv, q);
+    return (x == 0.f || fabsf(x) == INFINITY) ? x : x / d;
 }
 
-// g * dz/dx
-__device__ inline float sloped(const Row& w, float g, float xf, uint32_t count, bool ok) {
-    if (!ok) return 0.f;
-    if (!count) return g / w.temp;
-    const double s = xf > 0.f ? 1.0 / (double)w.rep : (double)w.rep;
-    return (float)((double)g * s / (double)w.temp);
+struct ProcessRow {
+    Row w;
+    double inv_temp;
+    float temp, inv_tempf;
+};
+template <bool RULES>
+__device__ inline ProcessRow process_row(const Rules& r, int64_t b) {
+    ProcessRow p;
+    p.w = row_of<RULES>(r, b);
+    p.inv_temp = 1.0 / p.w.temp;
+    p.temp = (float)p.w.temp;
+    p.inv_tempf = p.temp >= 0x1p-20f && p.temp <= 0x1p20f ? 1.f / p.temp : 0.f;
+    return p;
 }
 
+// z = y / T.  Under a temperature alone that is one correctly rounded float division; else y is a double, divided and rounded once.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock) process_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                          typename E::T* out, int64_t out_stride) {
-    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
-    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return row_of<RULES>(r, b); },
-                          [&](const Row& w, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
-        float v[kNv][E::kVec];
+    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    constexpr int C = E::kVec;
+    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
+                        [&](const ProcessRow& p, int64_t b, int64_t v0, int step, const uint32_t* c) {
+        Raw<E, C> raw[kNv];
 #pragma unroll
         for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);
+            if (k < t.nv && v0 + k * step < width) raw[k].load(x + b * stride, v0 + k * step, width);
 #pragma unroll
         for (int k = 0; k < kNv; k++) {
             const int64_t at = v0 + k * step;
             if (k >= t.nv || at >= width) continue;
-            const uint32_t bits = RULES ? allowed_bits(w, at) : 0xFFu;
+            float z[C];
+            if (RULES) {
+                double y[C];
+                ruled_cols(p.w, raw[k], at, width, c ? c + k * step : nullptr, y);
 #pragma unroll
-            for (int j = 0; j < E::kVec; j++)
-                v[k][j] = processed(w, v[k][j], c ? c[k * step + j] : 0u, bits >> j & 1, at + j < width ? at + j : 0);
-            store_cols<E>(out + b * out_stride, at, width, v[k]);
+                for (int j = 0; j < C; j++) z[j] = (float)divided(y[j], p.w.temp, p.inv_temp);
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; j++) z[j] = dividedf(raw[k].get(j), p.temp, p.inv_tempf);
+            }
+            raw[k].set(z);
+            raw[k].store(out + b * out_stride, at, width);
         }
     });
 }
 
+// g dz/dx.  Of the logit only its sign matters, and only under a penalty: a wave reads the logits of those vectors that hold a repeated id.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock) process_backward_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                                   const typename E::T* g, int64_t g_stride, typename E::T* out, int64_t out_stride) {
-    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
-    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return row_of<RULES>(r, b); },
-                          [&](const Row& w, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
-        float v[kNv][E::kVec], u[kNv][E::kVec];
+    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    constexpr int C = E::kVec;
+    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
+                        [&](const ProcessRow& p, int64_t b, int64_t v0, int step, const uint32_t* c) {
+        Raw<E, C> raw[kNv];
 #pragma unroll
         for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) {
-                load_cols<E>(g + b * g_stride, v0 + k * step, width, u[k], 0.f);
-                if (RULES && c) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);   // only its sign, and only under a penalty
-            }
+            if (k < t.nv && v0 + k * step < width) raw[k].load(g + b * g_stride, v0 + k * step, width);
 #pragma unroll
         for (int k = 0; k < kNv; k++) {
             const int64_t at = v0 + k * step;
             if (k >= t.nv || at >= width) continue;
-            const uint32_t bits = RULES ? allowed_bits(w, at) : 0xFFu;
+            float u[C];
 #pragma unroll
-            for (int j = 0; j < E::kVec; j++) u[k][j] = sloped(w, u[k][j], RULES && c ? v[k][j] : 0.f, RULES && c ? c[k * step + j] : 0u, bits >> j & 1);
-            store_cols<E>(out + b * out_stride, at, width, u[k]);
+            for (int j = 0; j < C; j++) u[j] = dividedf(raw[k].get(j), p.temp, p.inv_tempf);
+            if (RULES) {
+                const uint32_t bits = allowed_bits(p.w, at);
+                if (c) {
+                    uint32_t n[C], any = 0;
+#pragma unroll
+                    for (int j = 0; j < C; j++) any |= n[j] = c[k * step + j];
+                    if (any) {
+                        Raw<E, C> xs;
+                        xs.load(x + b * stride, at, width);
+#pragma unroll
+                        for (int j = 0; j < C; j++)
+                            if (n[j]) u[j] = (float)((double)raw[k].get(j) * (xs.get(j) > 0.f ? p.w.inv_rep : p.w.rep) * p.inv_temp);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < C; j++) u[j] = bits >> j & 1 ? u[j] : 0.f;
+            }
+            raw[k].set(u);
+            raw[k].store(out + b * out_stride, at, width);
         }
     });
 }
@@ -116,7 +147,7 @@ struct ScoreRow {
     Row w;
     int64_t act;
     double base;            // max y
-    float k, ls2, gl, ge, ent, inv_temp;
+    float k, ls2, gl, ge, ent, inv_temp, rep, inv_rep;
     bool empty;
 };
 
@@ -127,8 +158,9 @@ __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E
                                                                 const void* actions, int act64, const float* log_prob, const float* entropy,
                                                                 const double* log_sum, const float* g_lp, const float* g_ent,
                                                                 typename E::T* out, int64_t out_stride) {
-    __shared__ uint32_t counts[RULES ? kBlock * E::kVec * kNv : 1];
-    each_vector<E, RULES>(r, t, rows, width, counts, [&](int64_t b) {
+    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    constexpr int C = E::kVec;
+    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) {
         ScoreRow s;
         s.w = row_of<RULES>(r, b);
         s.act = act64 ? ((const int64_t*)actions)[b] : (int64_t)((const int32_t*)actions)[b];
@@ -136,39 +168,51 @@ __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E
         const double ls = log_sum[2 * b + 1];
         s.empty = ls == -INFINITY;
         s.ls2 = (float)(ls * kLog2e);
-        s.k = (float)(kLog2e / (double)s.w.temp);
+        s.inv_temp = (float)(1.0 / s.w.temp);
+        s.k = (float)(kLog2e / s.w.temp);
         s.gl = !g_lp || log_prob[b] == -INFINITY ? 0.f : g_lp[b];
         s.ge = g_ent ? g_ent[b] : 0.f;
         s.ent = entropy[b];
-        s.inv_temp = 1.f / s.w.temp;
+        s.rep = (float)s.w.rep;
+        s.inv_rep = (float)s.w.inv_rep;
         return s;
-    }, [&](const ScoreRow& s, int64_t b, int64_t v0, int64_t step, const uint32_t* c) {
-        float v[kNv][E::kVec];
+    }, [&](const ScoreRow& s, int64_t b, int64_t v0, int step, const uint32_t* c) {
+        Raw<E, C> raw[kNv];
 #pragma unroll
         for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) load_cols<E>(x + b * stride, v0 + k * step, width, v[k], 0.f);
+            if (k < t.nv && v0 + k * step < width) raw[k].load(x + b * stride, v0 + k * step, width);
 #pragma unroll
         for (int k = 0; k < kNv; k++) {
             const int64_t at = v0 + k * step;
             if (k >= t.nv || at >= width) continue;
             const uint32_t bits = s.empty ? 0u : RULES ? allowed_bits(s.w, at) : 0xFFu;
             const int64_t hot = s.act - at;
+            float g[C];
+            if (RULES) {
+                double y[C];
+                ruled_cols(s.w, raw[k], at, width, c ? c + k * step : nullptr, y);
 #pragma unroll
-            for (int j = 0; j < E::kVec; j++) {
-                const uint32_t n = RULES && c ? c[k * step + j] : 0u;
-                const float xf = v[k][j];
-                float d;
-                if (!RULES) d = xf - (float)s.base;   // the greatest logit: exact in float
-                else d = (float)(ruled(s.w, xf, n, true, at + j < width ? at + j : 0) - s.base);
-                const float lp2 = d * s.k - s.ls2;
+                for (int j = 0; j < C; j++) g[j] = (float)(y[j] - s.base);
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; j++) g[j] = raw[k].get(j) - (float)s.base;   // the greatest logit: exact in float
+            }
+#pragma unroll
+            for (int j = 0; j < C; j++) {
+                const float lp2 = __builtin_fmaf(g[j], s.k, -s.ls2);
                 const float p = __builtin_amdgcn_exp2f(lp2);
                 const float lp = (lp2 < -200.f ? -200.f : lp2) * (float)kLn2;   // p is 0 there; keeps 0 * inf out
-                float g = (hot == j ? s.gl : 0.f) - p * (s.gl + s.ge * (lp + s.ent));
-                g *= s.inv_temp;
-                if (RULES && n) g *= xf > 0.f ? 1.f / s.w.rep : s.w.rep;
-                v[k][j] = bits >> j & 1 ? g : 0.f;
+                g[j] = ((hot == j ? s.gl : 0.f) - p * __builtin_fmaf(s.ge, lp + s.ent, s.gl)) * s.inv_temp;
             }
-            store_cols<E>(out + b * out_stride, at, width, v[k]);
+            if (RULES && c) {
+#pragma unroll
+                for (int j = 0; j < C; j++)
+                    if (c[k * step + j]) g[j] *= raw[k].get(j) > 0.f ? s.inv_rep : s.rep;
+            }
+#pragma unroll
+            for (int j = 0; j < C; j++) g[j] = bits >> j & 1 ? g[j] : 0.f;
+            raw[k].set(g);
+            raw[k].store(out + b * out_stride, at, width);
         }
     });
 }

@@ -3,7 +3,7 @@
 // The action is the least column whose running sum of exp((y - max y) / T) passes u times the whole sum.  Everything that decides it is in
 // double: two neighbouring columns of a flat row of 2^17 lie 8e-6 of the sum apart, less than float32 sums of them are off by, and the same
 // logits must give the same action however the row is laid out and split.  Doubles run at the rate of floats here, and the exponential is
-// the 18 instructions of exp2_double.
+// the 16 instructions of exp2_double.
 #include "policy_common.h"
 
 namespace gymhip {
@@ -12,20 +12,79 @@ namespace {
 
 constexpr double kTiny = 0x1p-900;   // weights below count as none
 
-struct Choice {
-    int64_t at;   // the action's column, or -1
-    float log_prob;
-};
-
-__device__ inline double weight(double y, double base, double k) {
-    const double t = (y - base) * k;
-    return exp2_double(t > kLeast ? t : kLeast);   // -inf - base and its NaN cannot occur: base is finite
+// A weight against a finite base; NaN does not come here unmarked (see Tile::load).
+__device__ inline double weight(double y, double base, double k2) {
+    const double t = (y - base) * k2;
+    return exp2_double(t > kLeast ? t : kLeast);
 }
 
-// Which column of a group's tile the running sum passes `level` in; s[] are the sums of this lane's vectors.  Columns are in order of
-// (vector k, lane, element).  If rounding leaves the level above the last sum, the last column with any weight is taken.
-template <typename E, bool RULES, int G, int NV>
-__device__ inline int64_t locate(const Tile<E, RULES, NV>& tile, const double* s, double base, double k2, double level, double* lds, int* lds_at) {
+// One lane's share of a row's tile: NV vectors of C columns, `step` columns apart.  A vector is kept as it lies in memory, and gives its y
+// (float where y is the logit itself) each time it is gone through.
+template <typename E, bool RULES, int NV, int C>
+struct Tile {
+    using Y = typename std::conditional<RULES, double, float>::type;
+    Raw<E, C> raw[NV];
+
+    __device__ void load(const typename E::T* x, int64_t v0, int step, int64_t width) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) raw[k].load(x, v0 + k * step, NV == 1 || v0 + k * step < width ? width : v0 + k * step);
+    }
+    __device__ void get(int k, const Row& w, int64_t at, int64_t width, const uint32_t* counts, Y* y) const {
+        if constexpr (RULES) {
+            if (at < width) ruled_cols(w, raw[k], at, width, counts, y);
+            else
+#pragma unroll
+                for (int j = 0; j < C; j++) y[j] = -INFINITY;
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; j++) y[j] = raw[k].get(j);
+        }
+    }
+};
+
+// What a tile comes to: its greatest y, and the sum of its weights against that; `bad` where a NaN or +inf is among its y.
+// In s[k] the sums of this lane's vectors, against m.  Each vector is summed against its own maximum first, so that one pass over it does.
+template <typename E, bool RULES, int G, int NV, int C>
+__device__ inline void sum_tile(const Tile<E, RULES, NV, C>& tile, const Row& w, int64_t v0, int step, int64_t width, const uint32_t* counts, double k2,
+                                double* lds, double* s, double* m_out, double* sum_out, bool* bad_out) {
+    using Y = typename Tile<E, RULES, NV, C>::Y;
+    Y m[NV], top = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        Y y[C];
+        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
+        m[k] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            bad = bad || y[j] != y[j];
+            m[k] = y[j] > m[k] ? y[j] : m[k];
+        }
+        bad = bad || m[k] == INFINITY;
+        const double base = m[k] > -INFINITY && m[k] < INFINITY ? (double)m[k] : 0.0;
+        s[k] = 0;
+#pragma unroll
+        for (int j = 0; j < C; j++) s[k] += weight((double)y[j], base, k2);
+        top = m[k] > top ? m[k] : top;
+    }
+    top = group_reduce<G>(top, Max<Y>(), (Y*)lds);
+    const double base = top > -INFINITY && top < INFINITY ? (double)top : 0.0;
+    double sum = 0;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        if (!(NV == 1 && G == 1)) s[k] = m[k] > -INFINITY ? s[k] * weight((double)m[k], base, k2) : 0.0;
+        sum += s[k];
+    }
+    *sum_out = group_reduce<G>(sum, Sum<double>(), lds);
+    *m_out = (double)top;
+    *bad_out = group_reduce<G>((int)bad, Max<int>(), (int*)lds) != 0;
+}
+
+// Which column of a group's tile (0 = its first) the running sum passes `level` in; s[] as sum_tile leaves it, against `base`.  Columns are in
+// order of (vector k, lane, element).  If rounding leaves the level above the last sum, the last column with any weight is taken.
+template <typename E, bool RULES, int G, int NV, int C>
+__device__ inline int locate(const Tile<E, RULES, NV, C>& tile, const Row& w, int64_t v0, int step, int64_t width, const uint32_t* counts, const double* s,
+                             double base, double k2, double level, double* lds, int* lds_at) {
     constexpr int W = G < kWave ? G : kWave;           // lanes that exchange
     constexpr int M = G > kWave ? kBlock / kWave : 1;  // waves that share the tile
     const int lane = (int)threadIdx.x & (W - 1), wave = G > kWave ? (int)threadIdx.x / kWave : 0;
@@ -43,61 +102,50 @@ __device__ inline int64_t locate(const Tile<E, RULES, NV>& tile, const double* s
         for (int i = 0; i < NV * M; i++) sums[i] = lds[i];
     } else {
 #pragma unroll
-        for (int k = 0; k < NV; k++) sums[k] = group_reduce<G>(s[k], Sum<double>(), lds);
+        for (int k = 0; k < NV; k++) sums[k] = group_reduce<W>(s[k], Sum<double>(), lds);
     }
     // the part (vector, wave) that holds the level, and what comes before it
-    int part = -1;
+    int part = -1, some = 0;
     double before = 0;
 #pragma unroll
     for (int i = 0; i < NV * M; i++) {
-        const bool here = part < 0 && before + sums[i] > level;
-        if (here) part = i;
+        if (part < 0 && before + sums[i] > level) part = i;
         if (part < 0) before += sums[i];
+        if (sums[i] > kTiny) some = i;
     }
     if (part < 0) {
+        part = some;
         before = 0;
-#pragma unroll
-        for (int i = 0; i < NV * M; i++)
-            if (sums[i] > kTiny) part = i;
-        if (part < 0) part = 0;
         level = INFINITY;
     }
-    const int kk = part / M, ww = part - kk * M;
-    double sk = s[0];
-    typename Tile<E, RULES, NV>::Y y[E::kVec];
+    const int kk = NV == 1 ? 0 : __builtin_amdgcn_readfirstlane(part / M), ww = part - kk * M;   // NV > 1 has one row in a wave
+    int column = 0;
 #pragma unroll
-    for (int j = 0; j < E::kVec; j++) y[j] = tile.y[0][j];
+    for (int k = 0; k < NV; k++) {
+        if (NV > 1 && kk != k) continue;
+        const double upto = running_sum<W>(s[k], lane);
+        const int self = (int)(threadIdx.x & (kWave - 1));
+        const uint64_t group = W == 64 ? ~0ull : ((1ull << W) - 1) << (self & ~(W - 1));
+        const uint64_t hits = __ballot(s[k] > 0 && before + upto > level) & group, any = __ballot(s[k] > kTiny) & group;
+        const int first = hits ? __ffsll((unsigned long long)hits) - 1 : any ? 63 - __clzll((long long)any) : self;
+        // every lane walks its own vector; the chosen lane's answer counts
+        typename Tile<E, RULES, NV, C>::Y y[C];
+        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
+        double acc = before + (upto - s[k]);
+        int at = -1, last = 0;
 #pragma unroll
-    for (int k = 1; k < NV; k++)
-        if (kk == k) {
-            sk = s[k];
-#pragma unroll
-            for (int j = 0; j < E::kVec; j++) y[j] = tile.y[k][j];
+        for (int j = 0; j < C; j++) {
+            const double e = weight((double)y[j], base, k2);
+            acc += e;
+            if (e > kTiny) {
+                last = j;
+                if (at < 0 && acc > level) at = j;
+            }
         }
-    double upto = sk;
-#pragma unroll
-    for (int d = 1; d < W; d <<= 1) {
-        const double o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
+        if (at < 0) at = last;
+        if (W > 1) at = __shfl(at, first);
+        column = (k * G + (G > kWave ? ww * kWave : 0) + (first & (W - 1))) * C + at;
     }
-    const uint64_t group = W == 64 ? ~0ull : ((1ull << W) - 1) << ((int)(threadIdx.x & (kWave - 1)) & ~(W - 1));
-    const uint64_t hits = __ballot(sk > 0 && before + upto > level) & group, some = __ballot(sk > kTiny) & group;
-    const int first = hits ? __ffsll((unsigned long long)hits) - 1 : some ? 63 - __clzll((long long)some) : (int)(threadIdx.x & (kWave - 1));
-    // every lane walks its own vector; the chosen lane's answer counts
-    double acc = before + (upto - sk);
-    int at = -1, last = 0;
-#pragma unroll
-    for (int j = 0; j < E::kVec; j++) {
-        const double e = weight((double)y[j], base, k2);
-        acc += e;
-        if (e > kTiny) {
-            last = j;
-            if (at < 0 && acc > level) at = j;
-        }
-    }
-    if (at < 0) at = last;
-    at = __shfl(at, first);
-    int column = (kk * G + (ww * kWave) * (G > kWave) + (first & (W - 1))) * E::kVec + at;
     if (G > kWave) {
         if (wave == ww && lane == 0) *lds_at = column;
         __syncthreads();
@@ -106,26 +154,30 @@ __device__ inline int64_t locate(const Tile<E, RULES, NV>& tile, const double* s
     return column;
 }
 
-// The first column where the tile holds m, or `none`.
-template <typename E, bool RULES, int G, int NV>
-__device__ inline int64_t first_of(const Tile<E, RULES, NV>& tile, double m, int64_t v0, int64_t step, int64_t none, long long* lds) {
-    long long at = none;
+// The first column of the row where the tile holds m, or `none`.
+template <typename E, bool RULES, int G, int NV, int C>
+__device__ inline int64_t first_of(const Tile<E, RULES, NV, C>& tile, const Row& w, double m, int64_t v0, int step, int64_t width, const uint32_t* counts,
+                                   long long* lds) {
+    long long at = width;
 #pragma unroll
-    for (int k = NV - 1; k >= 0; k--)
+    for (int k = NV - 1; k >= 0; k--) {
+        typename Tile<E, RULES, NV, C>::Y y[C];
+        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
 #pragma unroll
-        for (int j = E::kVec - 1; j >= 0; j--)
-            if ((double)tile.y[k][j] == m) at = v0 + k * step + j;
+        for (int j = C - 1; j >= 0; j--)
+            if ((double)y[j] == m) at = v0 + k * step + j;
+    }
     return group_reduce<G>(at, Min<long long>(), lds);
 }
 
-__device__ inline float log_prob_of(const Row& w, double y, double m, double sum) { return (float)((y - m) / (double)w.temp - log(sum)); }
+__device__ inline float log_prob_of(double y, double m, double k2, double sum) { return (float)(((y - m) * k2 - log2_double(sum)) * kLn2); }
 
-// A row in G lanes' registers: rows of at most G * kVec * NV columns, kBlock / G of them per workgroup.
-template <typename E, bool RULES, int G, int NV>
+// A row in G lanes' registers: rows of at most G * C * NV columns, kBlock / G of them per workgroup.
+template <typename E, bool RULES, int G, int NV, int C>
 __global__ void __launch_bounds__(kBlock) sample_rows_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
                                                              int32_t* actions, float* log_prob) {
-    constexpr int per = kBlock / G, cap = G * E::kVec * NV;
-    __shared__ uint32_t counts[RULES ? per * cap : 1];
+    constexpr int per = kBlock / G, cap = G * C * NV, step = G * C;
+    __shared__ __align__(16) uint32_t counts[RULES ? per * cap : 4];
     __shared__ double lds[NV * (kBlock / kWave)];
     __shared__ long long lds_first[kBlock / kWave];
     __shared__ int lds_at;
@@ -137,38 +189,29 @@ __global__ void __launch_bounds__(kBlock) sample_rows_kernel(const typename E::T
         const int64_t b = own < rows ? own : rows - 1;   // lanes without a row follow the last one: every exchange has all its lanes
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const int64_t v0 = lane * E::kVec, step = (int64_t)G * E::kVec;
+        const int64_t v0 = lane * C;
         const uint32_t* mine = RULES && r.hist ? counts + group * cap : nullptr;
-        Tile<E, RULES, NV> tile;
+        const uint32_t* here = mine ? mine + v0 : nullptr;
+        Tile<E, RULES, NV, C> tile;
+        tile.load(x, v0, step, width);
+        const double u = row_uniform(keys, b);
+        const double k2 = kLog2e / w.temp;
+        double s[NV], m, sum;
         bool bad;
-        tile.load(w, x, v0, step, width, mine ? mine + v0 : nullptr, &bad);
-        using Y = typename Tile<E, RULES, NV>::Y;
-        const double m = (double)group_reduce<G>(tile.max(), Max<Y>(), (Y*)lds);
-        const int poison = group_reduce<G>((int)bad, Max<int>(), (int*)lds) | (m == INFINITY);
+        sum_tile<E, RULES, G, NV, C>(tile, w, v0, step, width, here, k2, lds, s, &m, &sum, &bad);
         const double base = m > -INFINITY && m < INFINITY ? m : 0.0;
-        const double k2 = kLog2e / (double)w.temp;
-        double s[NV], sum = 0;
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            s[k] = 0;
-#pragma unroll
-            for (int j = 0; j < E::kVec; j++) s[k] += weight((double)tile.y[k][j], base, k2);
-            sum += s[k];
-        }
-        sum = group_reduce<G>(sum, Sum<double>(), lds);
-        int64_t at = locate<E, RULES, G, NV>(tile, s, base, k2, row_uniform(keys, b) * sum, lds, &lds_at);
-        if (__syncthreads_or(w.greedy)) {
-            const int64_t first = first_of<E, RULES, G, NV>(tile, m, v0, step, width, lds_first);
+        int64_t at = locate<E, RULES, G, NV, C>(tile, w, v0, step, width, here, s, base, k2, u * sum, lds, &lds_at);
+        if (G > kWave ? w.greedy : __any(w.greedy)) {   // the same for all lanes that exchange
+            const int64_t first = first_of<E, RULES, G, NV, C>(tile, w, m, v0, step, width, here, lds_first);
             if (w.greedy) at = first;
         }
         if (lane == 0 && own < rows) {
-            float lp = poison ? NAN : -INFINITY;
-            if (poison || m == -INFINITY) at = -1;
-            else lp = log_prob_of(w, ruled(w, (float)x[at], mine ? mine[at] : 0u, true, at), m, sum);
+            float lp = bad ? NAN : -INFINITY;
+            if (bad || m == -INFINITY) at = -1;
+            else lp = log_prob_of(ruled(w, (float)x[at], mine ? mine[at] : 0u, true, at), m, k2, sum);
             actions[b] = (int32_t)at;
             log_prob[b] = lp;
         }
-        __syncthreads();
     }
 }
 
@@ -182,40 +225,31 @@ struct Part {
 template <typename E, bool RULES, int NV>
 __global__ void __launch_bounds__(kBlock) sample_parts_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int64_t cuts,
                                                               Part* parts) {
-    constexpr int cap = kBlock * E::kVec * NV;
-    __shared__ uint32_t counts[RULES ? cap : 1];
+    constexpr int C = E::kVec, cap = kBlock * C * NV, step = kBlock * C;
+    __shared__ __align__(16) uint32_t counts[RULES ? cap : 4];
     __shared__ double lds[kBlock / kWave];
     __shared__ long long lds_first[kBlock / kWave];
     for (int64_t i = blockIdx.x; i < rows * cuts; i += gridDim.x) {
         const int64_t b = i / cuts, lo = (i - b * cuts) * cap;
+        const int64_t v0 = lo + threadIdx.x * C;
+        Tile<E, RULES, NV, C> tile;
+        tile.load(x0 + b * stride, v0, step, width);
         if (RULES && r.hist) count_ids(r, b, 1, rows, width, lo, cap, counts);
+        const uint32_t* here = RULES && r.hist ? counts + threadIdx.x * C : nullptr;
         const Row w = row_of<RULES>(r, b);
-        const int64_t v0 = lo + threadIdx.x * E::kVec, step = (int64_t)kBlock * E::kVec;
-        Tile<E, RULES, NV> tile;
+        double s[NV], m, sum;
         bool bad;
-        tile.load(w, x0 + b * stride, v0, step, width, RULES && r.hist ? counts + threadIdx.x * E::kVec : nullptr, &bad);
-        using Y = typename Tile<E, RULES, NV>::Y;
-        const double m = (double)group_reduce<kBlock>(tile.max(), Max<Y>(), (Y*)lds);
-        const int poison = group_reduce<kBlock>((int)bad, Max<int>(), (int*)lds) | (m == INFINITY);
-        const double base = m > -INFINITY && m < INFINITY ? m : 0.0;
-        const double k2 = kLog2e / (double)w.temp;
-        double sum = 0;
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int j = 0; j < E::kVec; j++) sum += weight((double)tile.y[k][j], base, k2);
-        sum = group_reduce<kBlock>(sum, Sum<double>(), lds);
-        const int64_t first = w.greedy ? first_of<E, RULES, kBlock, NV>(tile, m, v0, step, width, lds_first) : 0;
-        if (threadIdx.x == 0) parts[i] = Part{m, poison ? (double)NAN : m == -INFINITY ? 0.0 : sum, first};
-        __syncthreads();
+        sum_tile<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, kLog2e / w.temp, lds, s, &m, &sum, &bad);
+        const int64_t first = w.greedy ? first_of<E, RULES, kBlock, NV, C>(tile, w, m, v0, step, width, here, lds_first) : 0;
+        if (threadIdx.x == 0) parts[i] = Part{m, bad ? (double)NAN : m == -INFINITY ? 0.0 : sum, first};
     }
 }
 
 template <typename E, bool RULES, int NV>
 __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
                                                              int64_t cuts, const Part* parts, int32_t* actions, float* log_prob) {
-    constexpr int cap = kBlock * E::kVec * NV;
-    __shared__ uint32_t counts[RULES ? cap : 1];
+    constexpr int C = E::kVec, cap = kBlock * C * NV, step = kBlock * C;
+    __shared__ __align__(16) uint32_t counts[RULES ? cap : 4];
     __shared__ double lds[NV * (kBlock / kWave)];
     __shared__ long long lds_first[kBlock / kWave];
     __shared__ int lds_at;
@@ -224,7 +258,7 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
     for (int64_t b = blockIdx.x; b < rows; b += gridDim.x) {
         const Part* p = parts + b * cuts;
         const Row w = row_of<RULES>(r, b);
-        const double k2 = kLog2e / (double)w.temp;
+        const double k2 = kLog2e / w.temp;
         double m = -INFINITY;
         int bad = 0;
         for (int64_t c = threadIdx.x; c < cuts; c += kBlock) {
@@ -260,12 +294,8 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
             for (int64_t c0 = 0; c0 < cuts; c0 += kBlock) {
                 const int64_t c = c0 + threadIdx.x;
                 const double e = share(c);
-                double upto = e;
                 const int lane = (int)threadIdx.x & (kWave - 1), wave = (int)threadIdx.x / kWave;
-                for (int d = 1; d < kWave; d <<= 1) {
-                    const double o = __shfl_up(upto, d);
-                    if (lane >= d) upto += o;
-                }
+                const double upto = running_sum<kWave>(e, lane);
                 __syncthreads();
                 if (lane == kWave - 1) lds[wave] = upto;
                 __syncthreads();
@@ -284,33 +314,27 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
                     break;
                 }
                 const long long most = group_reduce<kBlock>(e > 0 ? (long long)c : -1ll, Max<long long>(), lds_first);
-                if (most >= 0) {
-                    last = (int)most;
-                }
+                if (most >= 0) last = (int)most;
             }
             __syncthreads();
             const bool over = the_part < 0;
             const int c = over ? last : the_part;
-            const double target = over ? INFINITY : (level - before_part) / weight(p[c].m, m, k2);
-            const int64_t lo = (int64_t)c * cap;
+            const double top = p[c].m;
+            const double target = over ? INFINITY : (level - before_part) / weight(top, m, k2);
+            const int64_t lo = (int64_t)c * cap, v0 = lo + threadIdx.x * C;
+            Tile<E, RULES, NV, C> tile;
+            tile.load(x0 + b * stride, v0, step, width);
             if (RULES && r.hist) count_ids(r, b, 1, rows, width, lo, cap, counts);
-            Tile<E, RULES, NV> tile;
-            bool nan;
-            const int64_t v0 = lo + threadIdx.x * E::kVec, step = (int64_t)kBlock * E::kVec;
-            tile.load(w, x0 + b * stride, v0, step, width, RULES && r.hist ? counts + threadIdx.x * E::kVec : nullptr, &nan);
-            double s[NV];
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                s[k] = 0;
-#pragma unroll
-                for (int j = 0; j < E::kVec; j++) s[k] += weight((double)tile.y[k][j], p[c].m, k2);
-            }
-            at = lo + locate<E, RULES, kBlock, NV>(tile, s, p[c].m, k2, target, lds, &lds_at);
+            const uint32_t* here = RULES && r.hist ? counts + threadIdx.x * C : nullptr;
+            double s[NV], tile_m, tile_sum;
+            bool tile_bad;
+            sum_tile<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, k2, lds, s, &tile_m, &tile_sum, &tile_bad);
+            at = lo + locate<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, s, top, k2, target, lds, &lds_at);
         }
         if (threadIdx.x == 0) {
             const uint32_t n = RULES && r.hist ? counts[at % cap] : 0u;
             actions[b] = (int32_t)at;
-            log_prob[b] = log_prob_of(w, ruled(w, (float)x0[b * stride + at], n, true, at), m, sum);
+            log_prob[b] = log_prob_of(ruled(w, (float)x0[b * stride + at], n, true, at), m, k2, sum);
         }
         __syncthreads();
     }
@@ -329,11 +353,11 @@ size_t parts_bytes(int vec, int64_t rows, int64_t width) {
     return sizeof(Part) * (size_t)rows * (size_t)cuts_of(vec, wide_nv(vec, rows, width), width);
 }
 
-template <typename E, bool RULES, int G, int NV>
+template <typename E, bool RULES, int G, int NV, int C>
 void launch_rows(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const Keys& k, int32_t* actions, float* log_prob, hipStream_t s) {
     constexpr int per = kBlock / G;
-    hipLaunchKernelGGL((sample_rows_kernel<E, RULES, G, NV>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, (const typename E::T*)x, rows, width,
-                       stride, r, k, actions, log_prob);
+    hipLaunchKernelGGL((sample_rows_kernel<E, RULES, G, NV, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, (const typename E::T*)x, rows,
+                       width, stride, r, k, actions, log_prob);
 }
 
 template <typename E, bool RULES, int NV>
@@ -350,12 +374,17 @@ template <typename E, bool RULES>
 void launch(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const Keys& k, int32_t* actions, float* log_prob, void* ws,
             hipStream_t s) {
     constexpr int v = E::kVec;
-    if (width <= v) launch_rows<E, RULES, 1, 1>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 4 * v) launch_rows<E, RULES, 4, 1>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 16 * v) launch_rows<E, RULES, 16, 1>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 64 * v) launch_rows<E, RULES, 64, 1>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 64 * v * 4) launch_rows<E, RULES, 64, 4>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (!is_wide(v, width)) launch_rows<E, RULES, kBlock, 4>(x, rows, width, stride, r, k, actions, log_prob, s);
+    // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each
+    if (width <= 2) launch_rows<E, RULES, 1, 1, 2>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 4) launch_rows<E, RULES, 1, 1, 4>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= v) launch_rows<E, RULES, 1, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 2 * v) launch_rows<E, RULES, 2, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 4 * v) launch_rows<E, RULES, 4, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 8 * v) launch_rows<E, RULES, 8, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 16 * v) launch_rows<E, RULES, 16, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 64 * v) launch_rows<E, RULES, 64, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (width <= 64 * v * 4) launch_rows<E, RULES, 64, 4, v>(x, rows, width, stride, r, k, actions, log_prob, s);
+    else if (!is_wide(v, width)) launch_rows<E, RULES, kBlock, 4, v>(x, rows, width, stride, r, k, actions, log_prob, s);
     else if (wide_nv(v, rows, width) == 1) launch_wide<E, RULES, 1>(x, rows, width, stride, r, k, actions, log_prob, ws, s);
     else launch_wide<E, RULES, 4>(x, rows, width, stride, r, k, actions, log_prob, ws, s);
 }

@@ -1,7 +1,7 @@
 // policy_score.hip — log-probability and entropy of given actions under the ruled logits: one pass over the logits with a running maximum.
 //
 // With y the logit after penalties and bias, d = y - max y, t = d log2 e / T and w = 2^t:  S = sum w, D = sum w t,
-// log_prob = d_a / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to d, not to y); a thread adds up
+// log_prob = d_a / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to d, not to y); a lane adds up
 // at most 32 of them before it goes on in double.
 #include "policy_common.h"
 
@@ -26,29 +26,62 @@ __device__ inline void rebase(Run& r, double m, double k2) {
     r.m = m;
 }
 
-// One thread's tile added to its run.  NaN and +inf only mark it.
-template <typename E, bool RULES, int NV>
-__device__ inline void add_tile(Run& run, const Tile<E, RULES, NV>& tile, double m, double k2) {
-    using Y = typename Tile<E, RULES, NV>::Y;
-    if (!(m > -INFINITY && m < INFINITY)) {
-        if (m == INFINITY) run.bad = 1;
-        return;
+// C columns' y added to a run.  NaN and +inf only mark it.
+template <int C, typename Y>
+__device__ inline void add_cols(Run& run, const Y* y, double k2) {
+    Y m = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        bad = bad || y[j] != y[j];
+        m = y[j] > m ? y[j] : m;
     }
-    rebase(run, m, k2);
+    if (bad || m == INFINITY) run.bad = 1;
+    if (!(m < INFINITY)) return;
+    if ((double)m > run.m) rebase(run, (double)m, k2);
+    const double base = run.m > -INFINITY ? run.m : 0.0;
     const float k = (float)k2;
     float s = 0, d = 0;
 #pragma unroll
-    for (int q = 0; q < NV; q++)
-#pragma unroll
-        for (int j = 0; j < E::kVec; j++) {
-            float t = (float)(tile.y[q][j] - (Y)m) * k;
-            t = t > -200.f ? t : -200.f;   // 2^-200 is 0 in float32; keeps 0 * inf out
-            const float w = __builtin_amdgcn_exp2f(t);
-            s += w;
-            d = __builtin_fmaf(w, t, d);
-        }
+    for (int j = 0; j < C; j++) {
+        float t = (float)(y[j] - (Y)base) * k;
+        t = t > -200.f ? t : -200.f;   // 2^-200 is 0 in float32; keeps 0 * inf out
+        const float w = __builtin_amdgcn_exp2f(t);
+        s += w;
+        d = __builtin_fmaf(w, t, d);
+    }
     run.s += (double)s;
     run.d += (double)d;
+}
+
+// One lane's NV vectors of a tile added to its run: all loads first.  Logits without rules are summed 32 at a time, ruled ones by the vector
+// (their y are doubles, and 32 of them more registers than there are).
+template <typename E, bool RULES, int NV, int C>
+__device__ inline void add_tile(Run& run, const Row& w, const typename E::T* x, int64_t v0, int step, int64_t width, const Rules& r, int64_t b, int64_t lo,
+                                uint32_t* counts, const uint32_t* mine, double k2) {
+    Raw<E, C> raw[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) raw[k].load(x, v0 + k * step, NV == 1 || v0 + k * step < width ? width : v0 + k * step);
+    if constexpr (RULES) {
+        if (counts && r.hist) count_ids(r, b, 1, b + 1, width, lo, kBlock * C * NV, counts);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int64_t at = v0 + k * step;
+            double y[C];
+            if (at < width) ruled_cols(w, raw[k], at, width, mine ? mine + k * step : nullptr, y);
+            else
+#pragma unroll
+                for (int j = 0; j < C; j++) y[j] = -INFINITY;
+            add_cols<C>(run, y, k2);
+        }
+    } else {
+        float y[NV * C];
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < C; j++) y[k * C + j] = raw[k].get(j);
+        add_cols<NV * C>(run, y, k2);
+    }
 }
 
 // The group's run from its lanes'.
@@ -56,8 +89,7 @@ template <int G>
 __device__ inline void join(Run& run, double k2, double* lds) {
     const double m = group_reduce<G>(run.m, Max<double>(), lds);
     run.bad = group_reduce<G>(run.bad, Max<int>(), (int*)lds);
-    if (m > -INFINITY && m < INFINITY) rebase(run, m, k2);
-    run.m = m;
+    if (m > -INFINITY) rebase(run, m, k2);
     run.s = group_reduce<G>(run.s, Sum<double>(), lds);
     run.d = group_reduce<G>(run.d, Sum<double>(), lds);
 }
@@ -72,7 +104,7 @@ __device__ inline void finish(const Run& run, const Row& w, double ya, int64_t b
     }
     const bool empty = run.m == -INFINITY;
     const double ls = empty ? 0.0 : log(run.s);
-    log_prob[b] = empty ? -INFINITY : (float)((ya - run.m) / (double)w.temp - ls);
+    log_prob[b] = empty ? -INFINITY : (float)((ya - run.m) / w.temp - ls);
     entropy[b] = empty ? 0.f : (float)(ls - kLn2 * (run.d / run.s));
     log_sum[2 * b] = empty ? 0.0 : run.m;   // apart: beside a mask of the type's lowest value the sum of the two would lose log S
     log_sum[2 * b + 1] = empty ? -INFINITY : ls;
@@ -90,11 +122,11 @@ __device__ inline double y_at(const Row& w, const typename E::T* x, int64_t widt
     return ruled(w, (float)x[v], count ? *count : 0u, ok, v);
 }
 
-template <typename E, bool RULES, int G, int NV>
+template <typename E, bool RULES, int G, int NV, int C>
 __global__ void __launch_bounds__(kBlock) score_rows_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r,
                                                             const void* actions, int act64, float* log_prob, float* entropy, double* log_sum) {
-    constexpr int per = kBlock / G, cap = G * E::kVec * NV;
-    __shared__ uint32_t counts[RULES ? per * cap : 1];
+    constexpr int per = kBlock / G, cap = G * C * NV;
+    __shared__ __align__(16) uint32_t counts[RULES ? per * cap : 4];
     __shared__ double lds[kBlock / kWave];
     const int lane = (int)threadIdx.x & (G - 1);
     const int group = G >= kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : (int)threadIdx.x / G;
@@ -104,21 +136,15 @@ __global__ void __launch_bounds__(kBlock) score_rows_kernel(const typename E::T*
         const int64_t b = own < rows ? own : rows - 1;
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const int64_t v0 = lane * E::kVec;
         const uint32_t* mine = RULES && r.hist ? counts + group * cap : nullptr;
-        Tile<E, RULES, NV> tile;
-        bool bad;
-        tile.load(w, x, v0, (int64_t)G * E::kVec, width, mine ? mine + v0 : nullptr, &bad);
-        const double k2 = kLog2e / (double)w.temp;
-        using Y = typename Tile<E, RULES, NV>::Y;
-        Run run{-INFINITY, 0, 0, (int)bad};
-        add_tile<E, RULES, NV>(run, tile, (double)group_reduce<G>(tile.max(), Max<Y>(), (Y*)lds), k2);
+        const double k2 = kLog2e / w.temp;
+        Run run{-INFINITY, 0, 0, 0};
+        add_tile<E, RULES, NV, C>(run, w, x, lane * C, G * C, width, r, b, 0, nullptr, mine ? mine + lane * C : nullptr, k2);
         join<G>(run, k2, lds);
         if (lane == 0 && own < rows) {
             const int64_t a = action_of(actions, act64, b);
             finish(run, w, y_at<E>(w, x, width, a, mine && a >= 0 && a < width ? mine + a : nullptr), b, log_prob, entropy, log_sum);
         }
-        if (RULES) __syncthreads();
     }
 }
 
@@ -134,7 +160,7 @@ __global__ void __launch_bounds__(kBlock) score_wide_kernel(const typename E::T*
                                                             int splits, int64_t each, const void* actions, int act64, float* log_prob, float* entropy,
                                                             double* log_sum, Part* parts) {
     constexpr int cap = kBlock * E::kVec * kNv;
-    __shared__ uint32_t counts[RULES ? cap : 1];
+    __shared__ __align__(16) uint32_t counts[RULES ? cap : 4];
     __shared__ double lds[kBlock / kWave];
     __shared__ double the_ya;
     for (int64_t i = blockIdx.x; i < rows * splits; i += gridDim.x) {
@@ -143,20 +169,15 @@ __global__ void __launch_bounds__(kBlock) score_wide_kernel(const typename E::T*
         const int64_t c0 = part * each, c1 = c0 + each < cuts ? c0 + each : cuts;
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const double k2 = kLog2e / (double)w.temp;
+        const double k2 = kLog2e / w.temp;
         const int64_t a = action_of(actions, act64, b);
         Run run{-INFINITY, 0, 0, 0};
         if (threadIdx.x == 0) the_ya = -INFINITY;
         for (int64_t c = c0; c < c1; c++) {
             const int64_t lo = c * cap;
-            if (RULES && r.hist) count_ids(r, b, 1, rows, width, lo, cap, counts);
             const uint32_t* mine = RULES && r.hist ? counts : nullptr;
-            Tile<E, RULES, kNv> tile;
-            bool bad;
-            tile.load(w, x, lo + threadIdx.x * E::kVec, (int64_t)kBlock * E::kVec, width, mine ? mine + threadIdx.x * E::kVec : nullptr, &bad);
-            run.bad |= (int)bad;
-            const double m = (double)tile.max();
-            add_tile<E, RULES, kNv>(run, tile, m == INFINITY || run.m < m ? m : run.m, k2);
+            add_tile<E, RULES, kNv, E::kVec>(run, w, x, lo + threadIdx.x * E::kVec, kBlock * E::kVec, width, r, b, lo, counts,
+                                             mine ? mine + threadIdx.x * E::kVec : nullptr, k2);
             if (threadIdx.x == 0 && a >= lo && a < lo + cap) the_ya = y_at<E>(w, x, width, a, mine && a < width ? mine + (a - lo) : nullptr);
         }
         join<kBlock>(run, k2, lds);
@@ -178,7 +199,7 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
         const Row w = row_of<false>(r, b);
         Run run{-INFINITY, 0, 0, 0};
         if (lane < splits) run = parts[b * splits + lane].run;
-        join<kWave>(run, kLog2e / (double)w.temp, nullptr);
+        join<kWave>(run, kLog2e / w.temp, nullptr);
         if (lane == 0 && own < rows) {
             const int64_t a = action_of(actions, act64, b);
             finish(run, w, a >= 0 && a < width ? parts[b * splits + a / cap / each].ya : -INFINITY, b, log_prob, entropy, log_sum);
@@ -208,11 +229,11 @@ size_t parts_bytes(int vec, int64_t rows, int64_t width) {
     return splits == 1 ? 0 : sizeof(Part) * (size_t)rows * (size_t)splits;
 }
 
-template <typename E, bool RULES, int G, int NV>
+template <typename E, bool RULES, int G, int NV, int C>
 void launch_rows(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const void* actions, int act64, float* lp, float* ent, double* ls,
                  hipStream_t s) {
     constexpr int per = kBlock / G;
-    hipLaunchKernelGGL((score_rows_kernel<E, RULES, G, NV>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, (const typename E::T*)x, rows, width,
+    hipLaunchKernelGGL((score_rows_kernel<E, RULES, G, NV, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, (const typename E::T*)x, rows, width,
                        stride, r, actions, act64, lp, ent, ls);
 }
 
@@ -220,12 +241,16 @@ template <typename E, bool RULES>
 void launch(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const void* actions, int act64, float* lp, float* ent, double* ls,
             void* ws, hipStream_t s) {
     constexpr int v = E::kVec;
-    if (width <= v) return launch_rows<E, RULES, 1, 1>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
-    if (width <= 4 * v) return launch_rows<E, RULES, 4, 1>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
-    if (width <= 16 * v) return launch_rows<E, RULES, 16, 1>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
-    if (width <= 64 * v) return launch_rows<E, RULES, 64, 1>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
-    if (width <= 64 * v * 4) return launch_rows<E, RULES, 64, 4>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
-    if (!is_wide(v, width)) return launch_rows<E, RULES, kBlock, kNv>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 2) return launch_rows<E, RULES, 1, 1, 2>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 4) return launch_rows<E, RULES, 1, 1, 4>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= v) return launch_rows<E, RULES, 1, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 2 * v) return launch_rows<E, RULES, 2, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 4 * v) return launch_rows<E, RULES, 4, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 8 * v) return launch_rows<E, RULES, 8, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 16 * v) return launch_rows<E, RULES, 16, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 64 * v) return launch_rows<E, RULES, 64, 1, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (width <= 64 * v * 4) return launch_rows<E, RULES, 64, 4, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
+    if (!is_wide(v, width)) return launch_rows<E, RULES, kBlock, kNv, v>(x, rows, width, stride, r, actions, act64, lp, ent, ls, s);
     int splits;
     int64_t each;
     split(v, rows, width, &splits, &each);
