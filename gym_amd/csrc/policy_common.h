@@ -73,6 +73,45 @@ struct Raw {
         }
     }
     __device__ float get(int j) const { return E::widen(w, j); }
+    // get(j), and j set to v, for a j that is not known at compile time: by shifts, as a register has no index.
+    __device__ float pick(int j) const {
+        static_assert(kWords == 4, "");
+        const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+        constexpr int half = C / 2;
+        const uint32_t e[1] = {(uint32_t)((j & half ? hi : lo) >> ((j & (half - 1)) * (int)sizeof(T) * 8))};
+        return E::widen(e, 0);
+    }
+    __device__ void put(int j, float v) {
+        static_assert(kWords == 4, "");
+        constexpr int half = C / 2;
+        const float pair[2] = {v, 0.f};
+        const int shift = (j & (half - 1)) * (int)sizeof(T) * 8;
+        const uint64_t m = (sizeof(T) == 4 ? 0xFFFFFFFFull : 0xFFFFull) << shift, bits = (uint64_t)E::narrow(pair) << shift;
+        const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+        const uint64_t l = j & half ? lo : (lo & ~m) | (bits & m), h = j & half ? (hi & ~m) | (bits & m) : hi;
+        w[0] = (uint32_t)l;
+        w[1] = (uint32_t)(l >> 32);
+        w[2] = (uint32_t)h;
+        w[3] = (uint32_t)(h >> 32);
+    }
+    // All ones in the places of those elements of word i whose bit is set.
+    __device__ static uint32_t places(uint32_t bits, int i) {
+        if (sizeof(T) == 4) return (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 2 * i, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 2 * i + 1, 1);
+        return __builtin_amdgcn_perm(hi, lo, 0x05040100u);   // two bytes of each
+    }
+    // Elements whose bit is 0 become -inf, or 0.
+    __device__ void keep(uint32_t bits) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            const uint32_t m = places(bits, i);
+            w[i] = (w[i] & m) | (E::kNone & ~m);
+        }
+    }
+    __device__ void clear(uint32_t bits) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) w[i] &= places(bits, i);
+    }
     __device__ void set(const float* v) {
 #pragma unroll
         for (int i = 0; i < kWords; i++) w[i] = E::narrow(v + i * C / kWords);
@@ -146,7 +185,8 @@ struct Rules {
     int hist64, len64;
     const float *rep_rows, *pres_rows, *freq_rows, *temp_rows;
     float rep, pres, freq, temp;
-    __host__ __device__ bool plain() const { return !mask && !bias && !hist; }   // temperature alone
+    // y is the logit itself, or -inf where the mask does not allow it
+    __host__ __device__ bool plain() const { return !bias && !hist; }
 };
 
 // One row's share of them.
@@ -157,23 +197,24 @@ struct Row {
     bool greedy, nothing;   // nothing: its line lies behind the mask's last one
 };
 
+// RULES: there is a bias or a history.
 template <bool RULES>
 __device__ inline Row row_of(const Rules& r, int64_t b) {
     Row w;
     const float t = r.temp_rows ? r.temp_rows[b] : r.temp;
     w.greedy = !(t > 0.f);
-    w.temp = w.greedy ? 1.0 : (double)t;
+    w.temp = w.greedy ? 1.0 : t < 3e38f ? (double)t : 3e38;
     w.mask = nullptr;
     w.bias = nullptr;
     w.nothing = false;
     w.rep = w.inv_rep = 1.0;
     w.pres = w.freq = 0.0;
+    if (r.mask) {
+        const int64_t line = r.mask_rows ? r.mask_rows[b] : (r.mask_lines == 1 ? 0 : b);
+        w.nothing = line >= r.mask_lines;
+        if (line >= 0 && !w.nothing) w.mask = r.mask + line * r.mask_stride;
+    }
     if (RULES) {
-        if (r.mask) {
-            const int64_t line = r.mask_rows ? r.mask_rows[b] : (r.mask_lines == 1 ? 0 : b);
-            w.nothing = line >= r.mask_lines;
-            if (line >= 0 && !w.nothing) w.mask = r.mask + line * r.mask_stride;
-        }
         if (r.bias) w.bias = r.bias + b * r.bias_stride;
         if (r.hist) {
             w.rep = r.rep_rows ? r.rep_rows[b] : r.rep;
@@ -193,11 +234,14 @@ __device__ inline double divided(double x, double d, double inv) {
     return fabs(q) < INFINITY ? c : q;
 }
 
-// The mask's bits of C (at most 8) columns from v0 on, v0 a multiple of C and < width.
-__device__ inline uint32_t allowed_bits(const Row& w, int64_t v0) {
+// The mask's bits of C (at most 8) columns from v0 on, v0 a multiple of C; of none behind the row's end.
+__device__ inline uint32_t allowed_bits(const Row& w, int64_t v0, int64_t width) {
     if (w.nothing) return 0u;
-    return w.mask ? w.mask[v0 >> 5] >> (v0 & 31) : 0xFFu;
+    return w.mask && v0 < width ? w.mask[v0 >> 5] >> (v0 & 31) : 0xFFu;
 }
+
+__device__ inline bool has_mask(const Row& w) { return w.mask || w.nothing; }
+__device__ inline bool allowed(const Row& w, int64_t v) { return !w.nothing && (!w.mask || (w.mask[v >> 5] >> (v & 31) & 1u)); }
 
 // x under the penalties of a count > 0.
 __device__ inline double penalised(const Row& w, double x, uint32_t count) {
@@ -212,19 +256,83 @@ __device__ inline double ruled(const Row& w, float xf, uint32_t count, bool ok, 
     return ok ? y : -INFINITY;
 }
 
+// The biases of C columns from v0 on.
+template <int C>
+__device__ inline void bias_cols(const Row& w, int64_t v0, int64_t width, float* f) {
+    if (v0 + C <= width) {
+        struct __attribute__((packed, aligned(4))) Packed { float f[C]; };
+        const Packed p = *(const Packed*)(w.bias + v0);
+#pragma unroll
+        for (int j = 0; j < C; j++) f[j] = p.f[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; j++) f[j] = v0 + j < width ? w.bias[v0 + j] : 0.f;
+    }
+}
+
+// How often ids occur in a tile of columns of n rows, in LDS: 32 bits each, or 16 where no history is longer than 65,535; and with `bits` a bit for
+// each id that occurs at all, behind the counts (cap is a multiple of 32 then).
+struct Counts {
+    uint32_t* words;   // null: there is no history
+    int cap, all;      // columns of a row's tile; of all n rows'
+    bool half, bits;
+
+    __device__ uint32_t* touched() const { return words + (half ? all / 2 : all); }
+    __device__ int size() const { return (half ? all / 2 : all) + (bits ? all / 32 : 0); }
+    __device__ uint32_t at(int i) const { return half ? words[i >> 1] >> (16 * (i & 1)) & 0xFFFFu : words[i]; }
+    // C counts from i on, i a multiple of C.
+    template <int C>
+    __device__ void get(int i, uint32_t* c) const {
+        if (half) {
+#pragma unroll
+            for (int j = 0; j < C / 2; j++) {
+                const uint32_t v = words[i / 2 + j];
+                c[2 * j] = v & 0xFFFFu;
+                c[2 * j + 1] = v >> 16;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; j++) c[j] = words[i + j];
+        }
+    }
+    // Which of the C columns from i on have a count.
+    template <int C>
+    __device__ uint32_t which(int i) const {
+        if (bits) return touched()[i >> 5] >> (i & 31) & ((1u << C) - 1);
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < C; j++) m |= at(i + j) ? 1u << j : 0u;
+        return m;
+    }
+    // Whether any lane of the wave has a count among the columns of its vector at i (or it is not known without going through them).
+    template <int C>
+    __device__ bool any(int i) const { return words && (!bits || __any(which<C>(i))); }
+};
+
+// A vector as it is loaded: its columns, and the mask's bits for them.
+template <typename E, int C>
+struct Vector {
+    Raw<E, C> raw;
+    uint32_t bits;
+    __device__ void load(const Row& w, const typename E::T* row, int64_t at, int64_t width) {
+        raw.load(row, at, at < width ? width : 0);
+        bits = allowed_bits(w, at, width);
+    }
+};
+
 // y of C columns from v0 on: the logits after penalties and bias, before the temperature; -inf where the mask does not allow.  In double (which
 // runs at the rate of float here): what is compared and summed must be the formula's value even where a bias or a penalty cancels most of
-// the logit.  Straight-line code: a wave passes over the penalties only where none of its lanes has a count.
-// `counts`: the columns' counts, or null for the whole workgroup.
+// the logit.  Straight-line code: a wave passes over the penalties only where none of its lanes has a count (`counted` false, or found here).  bits: allowed_bits of the columns.
 template <typename E, int C>
-__device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, int64_t v0, int64_t width, const uint32_t* counts, double* y) {
-    const uint32_t bits = allowed_bits(w, v0);
+__device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, uint32_t bits, int64_t v0, int64_t width, const Counts& counts, int place, bool counted,
+                                  double* y) {
 #pragma unroll
     for (int j = 0; j < C; j++) y[j] = (double)raw.get(j);
-    if (counts) {
+    if (counted) {
         uint32_t c[C], any = 0;
+        counts.get<C>(place, c);
 #pragma unroll
-        for (int j = 0; j < C; j++) any |= c[j] = counts[j];
+        for (int j = 0; j < C; j++) any |= c[j];
         if (__any(any)) {
 #pragma unroll
             for (int j = 0; j < C; j++) {
@@ -235,15 +343,7 @@ __device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, int64_t v0
     }
     if (w.bias) {
         float f[C];
-        if (v0 + C <= width) {
-            struct __attribute__((packed, aligned(4))) Packed { float f[C]; };
-            const Packed p = *(const Packed*)(w.bias + v0);
-#pragma unroll
-            for (int j = 0; j < C; j++) f[j] = p.f[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < C; j++) f[j] = v0 + j < width ? w.bias[v0 + j] : 0.f;
-        }
+        bias_cols<C>(w, v0, width, f);
 #pragma unroll
         for (int j = 0; j < C; j++) y[j] += (double)f[j];
     }
@@ -251,34 +351,37 @@ __device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, int64_t v0
     for (int j = 0; j < C; j++) y[j] = bits >> j & 1 ? y[j] : -INFINITY;
 }
 
-// How often each id of columns [lo, lo + cap) occurs in the histories of rows [b0, b0 + n): counts[(row - b0) * cap + id - lo], by the whole
-// workgroup.  Integer LDS atomics, so their order is free.  Every thread of the workgroup comes here; counts may be read after it returns.
-// cap * n is a multiple of 4, counts 16-byte aligned.
+// Counts the ids of columns [lo, lo + cap) in the histories of rows [b0, b0 + n), n a power of two.  By the
+// whole workgroup: every thread comes here, and counts may be read after it returns.  Integer LDS atomics, so their order is free.
 template <typename Id>
-__device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_t span, int first, int step, uint32_t* counts) {
+__device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_t span, int first, int step, const Counts& c, int base) {
     struct __attribute__((packed, aligned(sizeof(Id)))) Four { Id v[4]; };
+    uint32_t* touched = c.touched();
+    auto count = [&](Id id) {
+        const uint64_t off = (uint64_t)((int64_t)id - lo);
+        if (off < span) {
+            const int at = base + (int)off;
+            if (c.half) atomicAdd(&c.words[at >> 1], 1u << (16 * (at & 1)));
+            else atomicAdd(&c.words[at], 1u);
+            if (c.bits) atomicOr(&touched[at >> 5], 1u << (at & 31));
+        }
+    };
     for (int64_t i = (int64_t)first * 4; i < len; i += (int64_t)step * 4) {
         if (i + 4 <= len) {
             const Four f = *(const Four*)(ids + i);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint64_t at = (uint64_t)((int64_t)f.v[j] - lo);
-                if (at < span) atomicAdd(&counts[at], 1u);
-            }
+            for (int j = 0; j < 4; j++) count(f.v[j]);
         } else {
-            for (int64_t j = i; j < len; j++) {
-                const uint64_t at = (uint64_t)((int64_t)ids[j] - lo);
-                if (at < span) atomicAdd(&counts[at], 1u);
-            }
+            for (int64_t j = i; j < len; j++) count(ids[j]);
         }
     }
 }
-__device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows, int64_t width, int64_t lo, int cap, uint32_t* counts) {
+__device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows, int64_t width, int64_t lo, const Counts& c) {
     __syncthreads();
-    for (int i = threadIdx.x; i < n * cap / 4; i += kBlock) ((uint4*)counts)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < c.size() / 4; i += kBlock) ((uint4*)c.words)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const uint32_t span = (uint32_t)(lo + cap < width ? cap : width - lo);
-    const int each = kBlock / n, mine = (int)threadIdx.x / each;   // n is a power of two: `each` adjacent threads take a row
+    const uint32_t span = (uint32_t)(lo + c.cap < width ? c.cap : width - lo);
+    const int each = kBlock / n, mine = (int)threadIdx.x / each;   // `each` adjacent threads take a row
     const int64_t b = b0 + mine;
     if (b < rows) {
         int64_t len = r.hist_cols;
@@ -287,11 +390,17 @@ __device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows
             len = have < len ? have : len;
         }
         const int first = (int)threadIdx.x & (each - 1);
-        if (r.hist64) count_row((const int64_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, counts + mine * cap);
-        else count_row((const int32_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, counts + mine * cap);
+        if (r.hist64) count_row((const int64_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, mine * c.cap);
+        else count_row((const int32_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, mine * c.cap);
     }
     __syncthreads();
 }
+
+// A workgroup's tile of columns is kTile 16-byte vectors a lane at most; half as many where the counts take 32 bits, so that both fit the same LDS.
+constexpr int kTile = 4;
+template <typename E>
+constexpr int counts_words() { return kBlock * E::kVec * kTile / 2 + kBlock * E::kVec * kTile / 32; }
+inline bool half_counts(const Rules& r) { return r.hist_cols <= 65535; }
 
 // ---- reductions over G lanes: G <= 64 adjacent lanes of a wave by lane permutations in the vector unit, G = kBlock through LDS as well --------
 template <int CTRL, int ROWS = 0xF>
@@ -341,36 +450,47 @@ __device__ inline double running_sum(double v, int lane) {
     return v;
 }
 
+// Orders what the lanes of a group have written to LDS before what they read.
+template <int G>
+__device__ inline void group_sync() {
+    if (G > kWave) {
+        __syncthreads();
+    } else {   // one wave's LDS accesses are in order: the compiler has to keep them so
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 template <typename V> struct Max { __device__ V operator()(V a, V b) const { return a > b ? a : b; } };   // of values without NaN
 template <typename V> struct Min { __device__ V operator()(V a, V b) const { return a < b ? a : b; } };
 template <typename V> struct Sum { __device__ V operator()(V a, V b) const { return a + b; } };
 
-// 2^t in double to 4e-16 of its value, for -1000 <= t <= 1000: t = n + f, |f| <= 1/2, and a polynomial of degree 10 through the Chebyshev nodes
-// for 2^f.  16 instructions, all at the double (= float) rate.
-__device__ inline double exp2_double(double t) {
-    const double shifted = t + 0x1.8p52;                                     // n in the low word
-    const double f = t - (shifted - 0x1.8p52);
-    double p = 0x1.e6063f7217bc6p-28;
-    p = __builtin_fma(p, f, 0x1.b675bca4eeebbp-24);
-    p = __builtin_fma(p, f, 0x1.62bfd47773353p-20);
-    p = __builtin_fma(p, f, 0x1.ffcb54062e698p-17);
-    p = __builtin_fma(p, f, 0x1.430913096fd9fp-13);
-    p = __builtin_fma(p, f, 0x1.5d87fe9d7a584p-10);
-    p = __builtin_fma(p, f, 0x1.3b2ab6fba1ddap-7);
-    p = __builtin_fma(p, f, 0x1.c6b08d703ce49p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
-    p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
-    p = __builtin_fma(p, f, 1.0);
+// 2^(d k) in double to 2e-14 of its value, for -1000 <= d k <= 1000: d k = n + f, |f| <= 1/2, and a polynomial of degree 9 through the Chebyshev
+// nodes for 2^f.  14 instructions, all at the double (= float) rate.
+__device__ inline double exp2_double(double d, double k) {
+    const double shifted = __builtin_fma(d, k, 0x1.8p52);                    // n in the low word
+    const double f = __builtin_fma(d, k, -(shifted - 0x1.8p52));
+    double p = 0x1.b6571de2f2351p-24;
+    p = __builtin_fma(p, f, 0x1.63ef969a64d3cp-20);
+    p = __builtin_fma(p, f, 0x1.ffcb76789860fp-17);
+    p = __builtin_fma(p, f, 0x1.43088e257f341p-13);
+    p = __builtin_fma(p, f, 0x1.5d87fe908f88ap-10);
+    p = __builtin_fma(p, f, 0x1.3b2ab72b175eep-7);
+    p = __builtin_fma(p, f, 0x1.c6b08d7044119p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbdff8149f2p-3);
+    p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
+    p = __builtin_fma(p, f, 0x1.000000000003dp+0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
 }
-// log2 s for 1 <= s < 2^100: the float logarithm l, and s 2^-l = 1 + e with |e| < 1e-6, whose logarithm is three terms of its series.
+// log2 s for a normal s: its exponent, and of its mantissa a the float logarithm l with a 2^-l = 1 + e, |e| < 1e-6, whose logarithm is three terms
+// of its series.
 __device__ inline double log2_double(double s) {
-    const double l = (double)__builtin_amdgcn_logf((float)s);
-    const double e = __builtin_fma(s, exp2_double(-l), -1.0);
-    return __builtin_fma(__builtin_fma(__builtin_fma(e, 1.0 / 3.0, -0.5), e, 1.0) * e, 1.4426950408889634074, l);
+    const int n = (int)(__double2hiint(s) >> 20) - 1023;
+    const double a = __hiloint2double((__double2hiint(s) & 0xFFFFF) | 0x3FF00000, __double2loint(s));
+    const double l = (double)__builtin_amdgcn_logf((float)a);
+    const double e = __builtin_fma(a, exp2_double(-l, 1.0), -1.0);
+    return __builtin_fma(__builtin_fma(__builtin_fma(e, 1.0 / 3.0, -0.5), e, 1.0) * e, 1.4426950408889634074, l) + (double)n;
 }
-// Below 2^-1000 a weight counts as none.
-constexpr double kLeast = -1000.0;
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 

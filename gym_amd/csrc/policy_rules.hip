@@ -5,46 +5,96 @@ namespace gymhip {
 namespace policy {
 namespace {
 
-// A workgroup takes a tile of R rows by C columns, C = lanes * kVec * NV with `lanes` a power of two: a row of at most kBlock * kVec * NV
+// A workgroup takes a tile of R rows by C columns, C = lanes * kVec * nv with `lanes` a power of two: a row of at most kBlock * kVec * kTile
 // columns is one tile's row (and several of them share a workgroup), a wider one is cut into tiles along its columns.
-// Each thread keeps NV 16-byte loads in flight.
-constexpr int kNv = 4;
-
 struct Tiling {
     int lanes_log2;      // lanes that share a row
-    int nv;              // vectors per lane, <= kNv
+    int nv;              // vectors a lane, <= kTile
     int64_t cuts;        // tiles along a row
     int64_t tiles;       // tiles in all
+    bool half;           // counts of 16 bits
 };
 
 template <typename E>
-Tiling tiling(int64_t rows, int64_t width) {
+Tiling tiling(int64_t rows, int64_t width, const Rules& r) {
     Tiling t;
+    t.half = half_counts(r);
     t.lanes_log2 = 0;
     while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) < width) t.lanes_log2++;
     const int64_t step = (int64_t)E::kVec << t.lanes_log2;
-    const int64_t need = (width + step - 1) / step;
-    t.nv = (int)(need < kNv ? need : kNv);
+    const int64_t need = (width + step - 1) / step, most = r.hist && !t.half ? kTile / 2 : kTile;
+    t.nv = (int)(need < most ? need : most);
     t.cuts = (width + step * t.nv - 1) / (step * t.nv);
     const int64_t per = kBlock >> t.lanes_log2;
     t.tiles = (rows + per - 1) / per * t.cuts;
     return t;
 }
 
-// Calls f(row state, row b, first column v0, columns from one of the lane's vectors to its next, counts at v0 or null) once per tile;
-// `begin(b)` makes the row's state.
+// Goes through a workgroup's tiles.  begin(b) makes a row's state; f(state, raw, b, first column, its mask bits, its place in the counts, apart) is called for
+// each of the lane's vectors of `src`, and changes raw into what is stored at `out`.  apart: which of its columns have a count, for f to go
+// through one by one after its straight pass over all.
+// Without rules all vectors are loaded first; under them it goes one at a time, with the next one's load under way, in fewer registers.
 template <typename E, bool RULES, typename Begin, typename F>
-__device__ inline void each_tile(const Rules& r, const Tiling& t, int64_t rows, int64_t width, uint32_t* counts, Begin begin, F f) {
-    const int lanes = 1 << t.lanes_log2, per = kBlock >> t.lanes_log2, cap = (E::kVec << t.lanes_log2) * t.nv;
+__device__ inline void each_vector(const Rules& r, const Tiling& t, const typename E::T* src, int64_t src_stride, int64_t rows, int64_t width,
+                                   typename E::T* out, int64_t out_stride, const Counts& counts, Begin begin, F f) {
+    constexpr int C = E::kVec;
+    const int lanes = 1 << t.lanes_log2, per = kBlock >> t.lanes_log2, step = C << t.lanes_log2, cap = counts.cap;
     const int mine = (int)threadIdx.x >> t.lanes_log2, lane = (int)threadIdx.x & (lanes - 1);
     for (int64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
         const int64_t band = t.cuts == 1 ? tile : tile / t.cuts;
         const int64_t lo = t.cuts == 1 ? 0 : (tile - band * t.cuts) * cap;
-        if (RULES && r.hist) count_ids(r, band * per, per, rows, width, lo, cap, counts);
-        const int64_t b = band * per + mine;
-        if (b < rows) f(begin(b), b, lo + lane * E::kVec, lanes * E::kVec, RULES && r.hist ? counts + mine * cap + lane * E::kVec : nullptr);
+        const int64_t b = band * per + mine, v0 = lo + lane * C, end = b < rows ? width : 0;
+        const int place = mine * cap + lane * C;
+        const typename E::T* from = src + b * src_stride;
+        typename E::T* to = out + b * out_stride;
+        if constexpr (RULES) {
+            Raw<E, C> next;
+            if (v0 < end) next.load(from, v0, width);
+            if (counts.words) count_ids(r, band * per, per, rows, width, lo, counts);
+            if (b >= rows) continue;
+            const auto state = begin(b);
+            uint32_t next_bits = allowed_bits(state, v0, width);
+#pragma unroll 1
+            for (int k = 0; k < t.nv; k++) {
+                const int64_t at = v0 + k * step;
+                if (at >= width) break;
+                const uint32_t apart = counts.words ? counts.which<C>(place + k * step) : 0u;
+                Raw<E, C> raw = next;
+                const uint32_t bits = next_bits;
+                if (k + 1 < t.nv && at + step < width) {
+                    next.load(from, at + step, width);
+                    next_bits = allowed_bits(state, at + step, width);
+                }
+                f(state, raw, b, at, bits, place + k * step, apart);
+                raw.store(to, at, width);
+            }
+        } else {
+            if (b >= rows) continue;
+            Raw<E, C> raw[kTile];
+            uint32_t bits[kTile];
+#pragma unroll
+            for (int k = 0; k < kTile; k++)
+                if (k < t.nv && v0 + k * step < width) raw[k].load(from, v0 + k * step, width);
+            const auto state = begin(b);
+            if (has_mask(state)) {
+#pragma unroll
+                for (int k = 0; k < kTile; k++) bits[k] = allowed_bits(state, v0 + k * step, width);
+            }
+#pragma unroll
+            for (int k = 0; k < kTile; k++) {
+                const int64_t at = v0 + k * step;
+                if (k >= t.nv || at >= width) continue;
+                f(state, raw[k], b, at, bits[k], 0, 0u);
+                raw[k].store(to, at, width);
+            }
+        }
     }
 }
+
+// The LDS of the counts, and what is in it.
+#define GYMHIP_POLICY_COUNTS(E, RULES)                                                      \
+    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];                  \
+    const Counts counts { RULES && r.hist ? words : nullptr, (E::kVec << t.lanes_log2) * t.nv, kBlock * E::kVec * t.nv, t.half, t.lanes_log2 >= 3 }
 
 // x / d of floats as IEEE rounds it.  inv = 1 / d, or 0 where d is not between 2^-20 and 2^20: then, and where the quotient is not between 2^-60 and
 // 2^100, the remainder may not be exact (see the double's `divided`) and the division itself is made.
@@ -54,166 +104,145 @@ __device__ inline float dividedf(float x, float d, float inv) {
     return (x == 0.f || fabsf(x) == INFINITY) ? x : x / d;
 }
 
-struct ProcessRow {
-    Row w;
+struct ProcessRow : Row {
     double inv_temp;
-    float temp, inv_tempf;
+    float tempf, inv_tempf;
 };
 template <bool RULES>
 __device__ inline ProcessRow process_row(const Rules& r, int64_t b) {
     ProcessRow p;
-    p.w = row_of<RULES>(r, b);
-    p.inv_temp = 1.0 / p.w.temp;
-    p.temp = (float)p.w.temp;
-    p.inv_tempf = p.temp >= 0x1p-20f && p.temp <= 0x1p20f ? 1.f / p.temp : 0.f;
+    (Row&)p = row_of<RULES>(r, b);
+    p.inv_temp = 1.0 / p.temp;
+    p.tempf = (float)p.temp;
+    p.inv_tempf = p.tempf >= 0x1p-20f && p.tempf <= 0x1p20f ? 1.f / p.tempf : 0.f;
     return p;
 }
 
-// z = y / T.  Under a temperature alone that is one correctly rounded float division; else y is a double, divided and rounded once.
+// z = y / T: one correctly rounded float division where y is the logit itself; under a penalty or a bias y is a double, divided and rounded once.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock) process_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                          typename E::T* out, int64_t out_stride) {
-    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    GYMHIP_POLICY_COUNTS(E, RULES);
     constexpr int C = E::kVec;
-    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
-                        [&](const ProcessRow& p, int64_t b, int64_t v0, int step, const uint32_t* c) {
-        Raw<E, C> raw[kNv];
+    each_vector<E, RULES>(r, t, x, stride, rows, width, out, out_stride, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
+                          [&](const ProcessRow& p, Raw<E, C>& raw, int64_t, int64_t at, uint32_t bits, int place, uint32_t apart) {
+        float z[C];
+        const Raw<E, C> whole = raw;
+        if (RULES && p.bias) {
+            float f[C];
+            bias_cols<C>(p, at, width, f);
 #pragma unroll
-        for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) raw[k].load(x + b * stride, v0 + k * step, width);
+            for (int j = 0; j < C; j++) z[j] = (float)divided((double)raw.get(j) + (double)f[j], p.temp, p.inv_temp);
+        } else {
 #pragma unroll
-        for (int k = 0; k < kNv; k++) {
-            const int64_t at = v0 + k * step;
-            if (k >= t.nv || at >= width) continue;
-            float z[C];
-            if (RULES) {
-                double y[C];
-                ruled_cols(p.w, raw[k], at, width, c ? c + k * step : nullptr, y);
-#pragma unroll
-                for (int j = 0; j < C; j++) z[j] = (float)divided(y[j], p.w.temp, p.inv_temp);
-            } else {
-#pragma unroll
-                for (int j = 0; j < C; j++) z[j] = dividedf(raw[k].get(j), p.temp, p.inv_tempf);
-            }
-            raw[k].set(z);
-            raw[k].store(out + b * out_stride, at, width);
+            for (int j = 0; j < C; j++) z[j] = dividedf(raw.get(j), p.tempf, p.inv_tempf);
         }
+        raw.set(z);
+        if (RULES) {
+            while (apart) {
+                const int j = __ffs((int)apart) - 1;
+                apart &= apart - 1;
+                raw.put(j, (float)divided(ruled(p, whole.pick(j), counts.at(place + j), true, at + j), p.temp, p.inv_temp));
+            }
+        }
+        if (has_mask(p)) raw.keep(bits);
     });
 }
 
-// g dz/dx.  Of the logit only its sign matters, and only under a penalty: a wave reads the logits of those vectors that hold a repeated id.
+// g dz/dx.  Of the logit only its sign matters, and only under a penalty: it is read for the columns with a count alone.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock) process_backward_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                                   const typename E::T* g, int64_t g_stride, typename E::T* out, int64_t out_stride) {
-    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    GYMHIP_POLICY_COUNTS(E, RULES);
     constexpr int C = E::kVec;
-    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
-                        [&](const ProcessRow& p, int64_t b, int64_t v0, int step, const uint32_t* c) {
-        Raw<E, C> raw[kNv];
+    each_vector<E, RULES>(r, t, g, g_stride, rows, width, out, out_stride, counts, [&](int64_t b) { return process_row<RULES>(r, b); },
+                          [&](const ProcessRow& p, Raw<E, C>& raw, int64_t b, int64_t at, uint32_t bits, int, uint32_t apart) {
+        float u[C];
+        const Raw<E, C> whole = raw;
 #pragma unroll
-        for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) raw[k].load(g + b * g_stride, v0 + k * step, width);
-#pragma unroll
-        for (int k = 0; k < kNv; k++) {
-            const int64_t at = v0 + k * step;
-            if (k >= t.nv || at >= width) continue;
-            float u[C];
-#pragma unroll
-            for (int j = 0; j < C; j++) u[j] = dividedf(raw[k].get(j), p.temp, p.inv_tempf);
-            if (RULES) {
-                const uint32_t bits = allowed_bits(p.w, at);
-                if (c) {
-                    uint32_t n[C], any = 0;
-#pragma unroll
-                    for (int j = 0; j < C; j++) any |= n[j] = c[k * step + j];
-                    if (any) {
-                        Raw<E, C> xs;
-                        xs.load(x + b * stride, at, width);
-#pragma unroll
-                        for (int j = 0; j < C; j++)
-                            if (n[j]) u[j] = (float)((double)raw[k].get(j) * (xs.get(j) > 0.f ? p.w.inv_rep : p.w.rep) * p.inv_temp);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < C; j++) u[j] = bits >> j & 1 ? u[j] : 0.f;
+        for (int j = 0; j < C; j++) u[j] = dividedf(raw.get(j), p.tempf, p.inv_tempf);
+        raw.set(u);
+        if (RULES) {
+            while (apart) {
+                const int j = __ffs((int)apart) - 1;
+                apart &= apart - 1;
+                const float xf = (float)x[b * stride + at + j];
+                raw.put(j, (float)((double)whole.pick(j) * (xf > 0.f ? p.inv_rep : p.rep) * p.inv_temp));
             }
-            raw[k].set(u);
-            raw[k].store(out + b * out_stride, at, width);
         }
+        if (has_mask(p)) raw.clear(bits);
     });
 }
 
-struct ScoreRow {
-    Row w;
+struct ScoreRow : Row {
     int64_t act;
     double base;            // max y
-    float k, ls2, gl, ge, ent, inv_temp, rep, inv_rep;
+    float k, ls2, gl, ge, ent, inv_temp, repf, inv_repf;
     bool empty;
+
+    // (delta gl - p (gl + ge (log p + H))) / T with p = 2^((y - max y) log2 e / T - log2 S), d = y - max y
+    __device__ float slope(float d, bool hot) const {
+        const float lp2 = __builtin_fmaf(d, k, -ls2);
+        const float p = __builtin_amdgcn_exp2f(lp2);
+        const float lp = (lp2 < -200.f ? -200.f : lp2) * (float)kLn2;   // p is 0 there; keeps 0 * inf out
+        return ((hot ? gl : 0.f) - p * __builtin_fmaf(ge, lp + ent, gl)) * inv_temp;
+    }
 };
 
-// dx = (delta gl - p (gl + ge (log p + H))) dz/dx with p = 2^((y - max y) log2 e / T - log2 S), in float32; y - max y is taken before anything is
-// rounded, so p is as exact far from 0 as near it.
+// dx = that times dy/dx, in float32; y - max y is taken before anything is rounded, so p is as exact far from 0 as near it.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                                 const void* actions, int act64, const float* log_prob, const float* entropy,
                                                                 const double* log_sum, const float* g_lp, const float* g_ent,
                                                                 typename E::T* out, int64_t out_stride) {
-    __shared__ __align__(16) uint32_t counts[RULES ? kBlock * E::kVec * kNv : 4];
+    GYMHIP_POLICY_COUNTS(E, RULES);
     constexpr int C = E::kVec;
-    each_tile<E, RULES>(r, t, rows, width, counts, [&](int64_t b) {
+    each_vector<E, RULES>(r, t, x, stride, rows, width, out, out_stride, counts, [&](int64_t b) {
         ScoreRow s;
-        s.w = row_of<RULES>(r, b);
+        (Row&)s = row_of<RULES>(r, b);
         s.act = act64 ? ((const int64_t*)actions)[b] : (int64_t)((const int32_t*)actions)[b];
         s.base = log_sum[2 * b];
         const double ls = log_sum[2 * b + 1];
         s.empty = ls == -INFINITY;
         s.ls2 = (float)(ls * kLog2e);
-        s.inv_temp = (float)(1.0 / s.w.temp);
-        s.k = (float)(kLog2e / s.w.temp);
+        s.inv_temp = (float)(1.0 / s.temp);
+        s.k = (float)(kLog2e / s.temp);
         s.gl = !g_lp || log_prob[b] == -INFINITY ? 0.f : g_lp[b];
         s.ge = g_ent ? g_ent[b] : 0.f;
         s.ent = entropy[b];
-        s.rep = (float)s.w.rep;
-        s.inv_rep = (float)s.w.inv_rep;
+        s.repf = (float)s.rep;
+        s.inv_repf = (float)s.inv_rep;
         return s;
-    }, [&](const ScoreRow& s, int64_t b, int64_t v0, int step, const uint32_t* c) {
-        Raw<E, C> raw[kNv];
+    }, [&](const ScoreRow& s, Raw<E, C>& raw, int64_t, int64_t at, uint32_t bits, int place, uint32_t apart) {
+        const int64_t hot = s.act - at;
+        float g[C];
+        const Raw<E, C> whole = raw;
+        if (RULES && s.bias) {
+            float f[C];
+            bias_cols<C>(s, at, width, f);
 #pragma unroll
-        for (int k = 0; k < kNv; k++)
-            if (k < t.nv && v0 + k * step < width) raw[k].load(x + b * stride, v0 + k * step, width);
+            for (int j = 0; j < C; j++) g[j] = (float)((double)raw.get(j) + (double)f[j] - s.base);
+        } else if (RULES) {
 #pragma unroll
-        for (int k = 0; k < kNv; k++) {
-            const int64_t at = v0 + k * step;
-            if (k >= t.nv || at >= width) continue;
-            const uint32_t bits = s.empty ? 0u : RULES ? allowed_bits(s.w, at) : 0xFFu;
-            const int64_t hot = s.act - at;
-            float g[C];
-            if (RULES) {
-                double y[C];
-                ruled_cols(s.w, raw[k], at, width, c ? c + k * step : nullptr, y);
+            for (int j = 0; j < C; j++) g[j] = (float)((double)raw.get(j) - s.base);
+        } else {
 #pragma unroll
-                for (int j = 0; j < C; j++) g[j] = (float)(y[j] - s.base);
-            } else {
-#pragma unroll
-                for (int j = 0; j < C; j++) g[j] = raw[k].get(j) - (float)s.base;   // the greatest logit: exact in float
-            }
-#pragma unroll
-            for (int j = 0; j < C; j++) {
-                const float lp2 = __builtin_fmaf(g[j], s.k, -s.ls2);
-                const float p = __builtin_amdgcn_exp2f(lp2);
-                const float lp = (lp2 < -200.f ? -200.f : lp2) * (float)kLn2;   // p is 0 there; keeps 0 * inf out
-                g[j] = ((hot == j ? s.gl : 0.f) - p * __builtin_fmaf(s.ge, lp + s.ent, s.gl)) * s.inv_temp;
-            }
-            if (RULES && c) {
-#pragma unroll
-                for (int j = 0; j < C; j++)
-                    if (c[k * step + j]) g[j] *= raw[k].get(j) > 0.f ? s.inv_rep : s.rep;
-            }
-#pragma unroll
-            for (int j = 0; j < C; j++) g[j] = bits >> j & 1 ? g[j] : 0.f;
-            raw[k].set(g);
-            raw[k].store(out + b * out_stride, at, width);
+            for (int j = 0; j < C; j++) g[j] = raw.get(j) - (float)s.base;   // the greatest logit: exact in float
         }
+#pragma unroll
+        for (int j = 0; j < C; j++) g[j] = s.slope(g[j], hot == j);
+        raw.set(g);
+        if (RULES) {
+            while (apart) {
+                const int j = __ffs((int)apart) - 1;
+                apart &= apart - 1;
+                const float xf = whole.pick(j);
+                const double y = ruled(s, xf, counts.at(place + j), true, at + j);
+                raw.put(j, s.slope((float)(y - s.base), hot == j) * (xf > 0.f ? s.inv_repf : s.repf));
+            }
+        }
+        if (s.empty) raw.clear(0u);
+        else if (has_mask(s)) raw.clear(bits);
     });
 }
 
@@ -322,7 +351,7 @@ int gymhip_process_logits(const void* logits, int type, int64_t rows, int64_t wi
         using E = decltype(e);
         using T = typename E::T;
         with_bool(!r.plain(), [&](auto ruled_) {
-            const Tiling t = tiling<E>(rows, width);
+            const Tiling t = tiling<E>(rows, width, r);
             hipLaunchKernelGGL((process_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream, (const T*)logits, rows,
                                width, stride, r, t, (T*)out, out_stride);
         });
@@ -342,7 +371,7 @@ int gymhip_process_logits_backward(const void* logits, int type, int64_t rows, i
         using E = decltype(e);
         using T = typename E::T;
         with_bool(!r.plain(), [&](auto ruled_) {
-            const Tiling t = tiling<E>(rows, width);
+            const Tiling t = tiling<E>(rows, width, r);
             hipLaunchKernelGGL((process_backward_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream,
                                (const T*)logits, rows, width, stride, r, t, (const T*)grad_out, grad_out_stride, (T*)grad_in, grad_in_stride);
         });
@@ -363,7 +392,7 @@ int gymhip_action_log_prob_backward(const void* logits, int type, int64_t rows, 
         using E = decltype(e);
         using T = typename E::T;
         with_bool(!r.plain(), [&](auto ruled_) {
-            const Tiling t = tiling<E>(rows, width);
+            const Tiling t = tiling<E>(rows, width, r);
             hipLaunchKernelGGL((score_backward_kernel<E, decltype(ruled_)::value>), dim3(grid_for(t.tiles)), dim3(kBlock), 0, (hipStream_t)stream,
                                (const T*)logits, rows, width, stride, r, t, actions, (int)(action_dtype == GYMHIP_ACT_I64), log_prob, entropy, log_sum,
                                grad_log_prob, grad_entropy, (T*)grad_in, grad_in_stride);

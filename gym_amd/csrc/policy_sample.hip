@@ -1,393 +1,551 @@
 // policy_sample.hip — one action per row from softmax of the ruled logits, and its log-probability.
 //
-// The action is the least column whose running sum of exp((y - max y) / T) passes u times the whole sum.  Everything that decides it is in
-// double: two neighbouring columns of a flat row of 2^17 lie 8e-6 of the sum apart, less than float32 sums of them are off by, and the same
-// logits must give the same action however the row is laid out and split.  Doubles run at the rate of floats here, and the exponential is
-// the 16 instructions of exp2_double.
+// The action is the least column whose running sum of exp(y / T) passes u times the whole sum.  Everything that decides it is in double: two
+// neighbouring columns of a flat row of 2^17 lie 8e-6 of the sum apart, about what float32 sums of them are off by, and the same logits must
+// give the same action however the row is laid out and split.  Doubles run at the rate of floats here (30e12 a second, measured), the
+// exponential is the 14 instructions of exp2_double, and a double's range lets one pass do without the maximum.
 #include "policy_common.h"
 
 namespace gymhip {
 namespace policy {
 namespace {
 
-constexpr double kTiny = 0x1p-900;   // weights below count as none
-
-// A weight against a finite base; NaN does not come here unmarked (see Tile::load).
-__device__ inline double weight(double y, double base, double k2) {
-    const double t = (y - base) * k2;
-    return exp2_double(t > kLeast ? t : kLeast);
+// What a row's temperature makes of the exponentials: a weight is 2^(d k2), d = y - base.  Below `least` it counts as none (2^-1000); up to
+// `most` it is at most 2^900.
+struct Scale {
+    double k2, least, most;
+};
+__device__ inline Scale scale_of(const Row& w) {
+    const double unit = w.temp * kLn2;
+    return Scale{kLog2e / w.temp, -1000.0 * unit, fmin(900.0 * unit, 3e38)};   // an infinite logit never fits
 }
+__device__ inline double weight(double d, const Scale& c) { return exp2_double(__builtin_fmax(d, c.least), c.k2); }
 
-// One lane's share of a row's tile: NV vectors of C columns, `step` columns apart.  A vector is kept as it lies in memory, and gives its y
-// (float where y is the logit itself) each time it is gone through.
-template <typename E, bool RULES, int NV, int C>
-struct Tile {
-    using Y = typename std::conditional<RULES, double, float>::type;
-    Raw<E, C> raw[NV];
+// Where a lane stands in its row: `at` its first column, `step` the columns from one of its vectors to the next, `place` its first column's place in
+// the counts.
+struct Place {
+    int64_t at, width;
+    int step, place;
+    Counts counts;   // words null: no history
 
-    __device__ void load(const typename E::T* x, int64_t v0, int step, int64_t width) {
-#pragma unroll
-        for (int k = 0; k < NV; k++) raw[k].load(x, v0 + k * step, NV == 1 || v0 + k * step < width ? width : v0 + k * step);
-    }
-    __device__ void get(int k, const Row& w, int64_t at, int64_t width, const uint32_t* counts, Y* y) const {
-        if constexpr (RULES) {
-            if (at < width) ruled_cols(w, raw[k], at, width, counts, y);
-            else
-#pragma unroll
-                for (int j = 0; j < C; j++) y[j] = -INFINITY;
-        } else {
-#pragma unroll
-            for (int j = 0; j < C; j++) y[j] = raw[k].get(j);
-        }
-    }
+    __device__ bool inside(int k) const { return at + k * step < width; }
 };
 
-// What a tile comes to: its greatest y, and the sum of its weights against that; `bad` where a NaN or +inf is among its y.
-// In s[k] the sums of this lane's vectors, against m.  Each vector is summed against its own maximum first, so that one pass over it does.
-template <typename E, bool RULES, int G, int NV, int C>
-__device__ inline void sum_tile(const Tile<E, RULES, NV, C>& tile, const Row& w, int64_t v0, int step, int64_t width, const uint32_t* counts, double k2,
-                                double* lds, double* s, double* m_out, double* sum_out, bool* bad_out) {
-    using Y = typename Tile<E, RULES, NV, C>::Y;
-    Y m[NV], top = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-        Y y[C];
-        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
-        m[k] = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < C; j++) {
-            bad = bad || y[j] != y[j];
-            m[k] = y[j] > m[k] ? y[j] : m[k];
+// f(y) for the y of vector k: floats where they are the logits themselves, else (under a bias, or where a lane of the wave has a count) doubles.
+template <typename E, bool RULES, int C, typename F>
+__device__ inline void with_y(const Row& w, const Place& p, int k, Vector<E, C> v, F f) {
+    if constexpr (RULES) {
+        const bool counted = p.counts.any<C>(p.place + k * p.step);
+        if (counted || w.bias) {
+            double y[C];
+            ruled_cols(w, v.raw, v.bits, p.at + k * p.step, p.width, p.counts, p.place + k * p.step, counted, y);
+            f(y);
+            return;
         }
-        bad = bad || m[k] == INFINITY;
-        const double base = m[k] > -INFINITY && m[k] < INFINITY ? (double)m[k] : 0.0;
-        s[k] = 0;
-#pragma unroll
-        for (int j = 0; j < C; j++) s[k] += weight((double)y[j], base, k2);
-        top = m[k] > top ? m[k] : top;
     }
-    top = group_reduce<G>(top, Max<Y>(), (Y*)lds);
-    const double base = top > -INFINITY && top < INFINITY ? (double)top : 0.0;
-    double sum = 0;
+    if (has_mask(w)) v.raw.keep(v.bits);
+    float y[C];
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        if (!(NV == 1 && G == 1)) s[k] = m[k] > -INFINITY ? s[k] * weight((double)m[k], base, k2) : 0.0;
-        sum += s[k];
-    }
-    *sum_out = group_reduce<G>(sum, Sum<double>(), lds);
-    *m_out = (double)top;
-    *bad_out = group_reduce<G>((int)bad, Max<int>(), (int*)lds) != 0;
+    for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
+    f(y);
 }
 
-// Which column of a group's tile (0 = its first) the running sum passes `level` in; s[] as sum_tile leaves it, against `base`.  Columns are in
-// order of (vector k, lane, element).  If rounding leaves the level above the last sum, the last column with any weight is taken.
-template <typename E, bool RULES, int G, int NV, int C>
-__device__ inline int locate(const Tile<E, RULES, NV, C>& tile, const Row& w, int64_t v0, int step, int64_t width, const uint32_t* counts, const double* s,
-                             double base, double k2, double level, double* lds, int* lds_at) {
-    constexpr int W = G < kWave ? G : kWave;           // lanes that exchange
-    constexpr int M = G > kWave ? kBlock / kWave : 1;  // waves that share the tile
-    const int lane = (int)threadIdx.x & (W - 1), wave = G > kWave ? (int)threadIdx.x / kWave : 0;
-    double sums[NV * M];
-    if (G > kWave) {
-        __syncthreads();
+// A vector's weights e against `base`, and their sum.
+template <int C, typename Y>
+__device__ inline double weigh(const Y* y, double base, const Scale& c, double* e) {
+    double s = 0;
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const double t = group_reduce<kWave>(s[k], Sum<double>(), lds);
-            if (lane == 0) lds[k * M + wave] = t;
-        }
-        if (threadIdx.x == 0) *lds_at = 0;
-        __syncthreads();
+    for (int j = 0; j < C; j++) s += e[j] = weight((double)y[j] - base, c);
+    return s;
+}
+// The same against 0.  A double holds 2^-900 .. 2^900 at full precision, so nothing has to be known of the greatest y beforehand: this is all there
+// is to do where no y is above `most` nor a NaN and the row's sum is not below 2^-900.  *beyond: the wave's lanes that have such a y (as a lane mask: one
+// vector instruction a column).
+template <int C, typename Y>
+__device__ inline double weigh_0(const Y* y, const Scale& c, double* e, uint64_t* beyond) {
+    double s = 0;
 #pragma unroll
-        for (int i = 0; i < NV * M; i++) sums[i] = lds[i];
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; k++) sums[k] = group_reduce<W>(s[k], Sum<double>(), lds);
+    for (int j = 0; j < C; j++) {
+        *beyond |= __ballot(!(y[j] <= (Y)c.most));
+        s += e[j] = weight((double)y[j], c);
     }
+    return s;
+}
+// The sum of vector k's weights against 0, in no order of columns: the few columns with a count are left out of the straight pass, which then is no
+// dearer than one without a history, and each is gone through by itself afterwards by the lane that owns it.
+template <typename E, bool RULES>
+__device__ inline double weigh_apart(const Row& w, const Place& p, int k, Vector<E, E::kVec> v, const Scale& c, uint64_t* beyond) {
+    constexpr int C = E::kVec;
+    double e[C];
+    if constexpr (!RULES) {
+        double s = 0;
+        with_y<E, false, C>(w, p, k, v, [&](const auto* y) { s = weigh_0<C>(y, c, e, beyond); });
+        return s;
+    } else {
+        const int64_t at = p.at + k * p.step;
+        const int place = p.place + k * p.step;
+        uint32_t apart = p.counts.words ? p.counts.which<C>(place) & v.bits : 0u;
+        const Raw<E, C> whole = v.raw;
+        if (has_mask(w) || __any(apart)) v.raw.keep(v.bits & ~apart);
+        double s;
+        if (w.bias) {
+            float f[C];
+            double y[C];
+            bias_cols<C>(w, at, p.width, f);
+#pragma unroll
+            for (int j = 0; j < C; j++) y[j] = (double)v.raw.get(j) + (double)f[j];
+            s = weigh_0<C>(y, c, e, beyond);
+        } else {
+            float y[C];
+#pragma unroll
+            for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
+            s = weigh_0<C>(y, c, e, beyond);
+        }
+        while (apart) {
+            const int j = __ffs((int)apart) - 1;
+            apart &= apart - 1;
+            const double y = ruled(w, whole.pick(j), p.counts.at(place + j), true, at + j);
+            s += weigh_0<1>(&y, c, e, beyond);
+        }
+        return s;
+    }
+}
+__device__ inline bool mine_in(uint64_t lanes) { return lanes >> (threadIdx.x & (kWave - 1)) & 1; }
+
+// The sum of a group's weights against `base`; bad: a NaN or +inf is among its y.
+struct Mass {
+    double base, sum;
+    bool bad;
+};
+
+// The greatest y of a group's columns (nv vectors a lane), whatever it is (-inf: there is none at all), the sum against it, and the first column that
+// holds it: for greedy rows, and the rare ones out of weigh_0's range.
+template <typename E, bool RULES, int G, int C>
+__device__ inline Mass sum_against_max(const typename E::T* x, const Row& w, const Place& p, int nv, const Scale& c, double* lds, long long* first) {
+    double m = -INFINITY, sum = 0;
+    int best = 0;
+    bool bad = false;
+#pragma unroll 1
+    for (int k = 0; k < nv; k++) {
+        Vector<E, C> v;
+        v.load(w, x, p.at + k * p.step, p.width);
+        with_y<E, RULES, C>(w, p, k, v, [&](const auto* y) {
+            auto top = y[0];
+            bool nan = top != top;
+#pragma unroll
+            for (int j = 1; j < C; j++) {
+                nan = nan || y[j] != y[j];
+                top = y[j] > top || top != top ? y[j] : top;
+            }
+            if (nan || top == INFINITY) bad = true;
+            if (nan || !(top > -INFINITY && top < INFINITY)) return;
+            if ((double)top > m) {   // never from -inf with a sum
+                sum = sum > 0 ? sum * weight(m - (double)top, c) : 0.0;
+                m = (double)top;
+                best = k;
+            }
+            double e[C];
+            sum += weigh<C>(y, m, c, e);
+        });
+    }
+    const double top = group_reduce<G>(m, Max<double>(), lds);
+    sum = m > -INFINITY ? sum * weight(m - top, c) : 0.0;
+    Mass mass;
+    mass.base = top;
+    mass.sum = group_reduce<G>(sum, Sum<double>(), lds);
+    mass.bad = group_reduce<G>((int)bad, Max<int>(), (int*)lds) != 0;
+    long long at = p.width;
+    if (__any(w.greedy)) {   // each lane's first greatest, of which its vector is known
+        Vector<E, C> v;
+        v.load(w, x, p.at + best * p.step, p.width);
+        with_y<E, RULES, C>(w, p, best, v, [&](const auto* y) {
+#pragma unroll
+            for (int j = C - 1; j >= 0; j--)
+                if ((double)y[j] == top) at = p.at + best * p.step + j;
+        });
+    }
+    *first = group_reduce<G>(at, Min<long long>(), (long long*)lds);
+    return mass;
+}
+
+// The column (0 = the first of the lanes' vectors) of W lanes' vectors that the running sum passes `level` in: e[] a lane's weights, s their sum.
+// Should rounding leave the level above all sums, the last column with any weight is taken; weights up to `tiny` count as none to that.
+template <int W, int C>
+__device__ inline int walk(const double* e, double s, double before, double level, double tiny) {
+    const int self = (int)(threadIdx.x & (kWave - 1)), lane = self & (W - 1);
+    const double upto = running_sum<W>(s, lane);
+    int first = self;
+    if (W > 1) {
+        const uint64_t group = W == 64 ? ~0ull : ((1ull << W) - 1) << (self & ~(W - 1));
+        const uint64_t hits = __ballot(s > 0 && before + upto > level) & group, any = __ballot(s > tiny) & group;
+        first = hits ? __ffsll((unsigned long long)hits) - 1 : any ? 63 - __clzll((long long)any) : self;
+    }
+    // every lane walks its own vector; the chosen lane's answer counts
+    double acc = before + (upto - s);
+    int at = -1, last = 0;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        acc += e[j];
+        if (e[j] > tiny) {
+            last = j;
+            if (at < 0 && acc > level) at = j;
+        }
+    }
+    if (at < 0) at = last;
+    if (W > 1) at = __shfl(at, first);
+    return (first & (W - 1)) * C + at;
+}
+
+__device__ inline float log_prob_of(double y, double m, double k2, double sum) { return (float)(((y - m) * k2 - log2_double(sum)) * kLn2); }
+
+// A row's answer, by one lane: `at` its chosen column unless there is none.
+template <typename E>
+__device__ inline void answer(const Row& w, const typename E::T* x, const Mass& mass, int64_t at, uint32_t count, const Scale& c, int64_t b,
+                              int32_t* actions, float* log_prob) {
+    const bool none = mass.bad || mass.base == -INFINITY;
+    actions[b] = none ? -1 : (int32_t)at;
+    log_prob[b] = mass.bad ? NAN : none ? -INFINITY : log_prob_of(ruled(w, (float)x[at], count, true, at), mass.base, c.k2, mass.sum);
+}
+
+// Rows of at most G * C columns, G <= 64: one vector a lane, kBlock / G rows per workgroup.
+template <typename E, bool RULES, int G, int C>
+__global__ void __launch_bounds__(kBlock) sample_vectors_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
+                                                                int32_t* actions, float* log_prob) {
+    constexpr int per = kBlock / G, cap = G * C;
+    __shared__ __align__(16) uint32_t words[RULES ? per * cap : 4];
+    const int lane = (int)threadIdx.x & (G - 1);
+    const int group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : (int)threadIdx.x / G;
+    const bool hist = RULES && r.hist;
+    const Counts counts{hist ? words : nullptr, cap, per * cap, false, false};
+    for (int64_t band = blockIdx.x; band * per < rows; band += gridDim.x) {
+        const int64_t own = band * per + group;
+        const int64_t b = own < rows ? own : rows - 1;   // lanes without a row follow the last one: every exchange has all its lanes
+        const Row w = row_of<RULES>(r, b);
+        const typename E::T* x = x0 + b * stride;
+        const Place p{lane * C, width, G * C, group * cap + lane * C, counts};
+        Vector<E, C> v;
+        v.load(w, x, p.at, width);
+        if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
+        const Scale c = scale_of(w);
+        double s = 0, e[C];
+        uint64_t beyond = 0;
+        with_y<E, RULES, C>(w, p, 0, v, [&](const auto* y) { s = weigh_0<C>(y, c, e, &beyond); });
+        Mass mass{0.0, group_reduce<G>(w.greedy || mine_in(beyond) ? (double)NAN : s, Sum<double>(), (double*)nullptr), false};
+        const bool whole = mass.sum > 0x1p-900;
+        long long first = 0;
+        if (__any(!whole)) {   // the same for all lanes that exchange
+            const Mass other = sum_against_max<E, RULES, G, C>(x, w, p, 1, c, nullptr, &first);
+            if (!whole) {
+                mass = other;
+                const double base = mass.base > -INFINITY ? mass.base : 0.0;
+                with_y<E, RULES, C>(w, p, 0, v, [&](const auto* y) { s = weigh<C>(y, base, c, e); });
+            }
+        }
+        int64_t at = walk<G, C>(e, s, 0.0, row_uniform(keys, b) * mass.sum, mass.sum * 0x1p-80);
+        if (w.greedy) at = first;
+        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? words[group * cap + at] : 0u, c, b, actions, log_prob);
+    }
+}
+
+// A strip of a row: the columns of G = 64 or kBlock lanes, nv <= kTile vectors each, gone through one vector at a time with the next one's load
+// under way: few registers, so that many waves are there to wait for memory and for the workgroup's barriers.
+template <typename E, typename F>
+__device__ inline void each_vector(const Row& w, const typename E::T* x, const Place& p, int nv, Vector<E, E::kVec> next, F f) {
+#pragma unroll 1
+    for (int k = 0; k < nv; k++) {
+        const Vector<E, E::kVec> v = next;
+        if (k + 1 < nv) next.load(w, x, p.at + (k + 1) * p.step, p.width);
+        f(k, v);
+    }
+}
+
+// sums[k * waves + wave]: the sum of each wave's k-th vectors against `base`.  v0: this lane's first vector.
+template <typename E, bool RULES, int G>
+__device__ inline void strip_sums(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Scale& c, double base,
+                                  double* sums) {
+    constexpr int C = E::kVec, M = G / kWave;
+    const int wave = G > kWave ? (int)threadIdx.x / kWave : 0;
+    group_sync<G>();
+    each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) {
+        double s = 0, e[C];
+        with_y<E, RULES, C>(w, p, k, v, [&](const auto* y) { s = weigh<C>(y, base, c, e); });
+        s = group_reduce<kWave>(s, Sum<double>(), (double*)nullptr);
+        if ((threadIdx.x & (kWave - 1)) == 0) sums[k * M + wave] = s;
+    });
+    group_sync<G>();
+}
+
+// The sum of a strip.
+template <typename E, bool RULES, int G>
+__device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Scale& c, double* lds,
+                                 long long* first) {
+    constexpr int C = E::kVec;
+    if (!w.greedy) {   // one row's: all lanes alike
+        double sum = 0;
+        uint64_t beyond = 0;
+        each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) { sum += weigh_apart<E, RULES>(w, p, k, v, c, &beyond); });
+        const Mass mass{0.0, group_reduce<G>(mine_in(beyond) ? (double)NAN : sum, Sum<double>(), lds), false};
+        if (mass.sum > 0x1p-900) return mass;
+    }
+    return sum_against_max<E, RULES, G, C>(x, w, p, nv, c, lds, first);
+}
+
+// The column of a strip (0 = its first) that the running sum passes `level` in; sums as strip_sums left them for the same base, which is finite, and
+// `sum` the strip's.
+template <typename E, bool RULES, int G>
+__device__ inline int locate(const typename E::T* x, const Row& w, const Place& p, int nv, const Scale& c, double base, double sum, double level,
+                             const double* sums, int* lds_at) {
+    constexpr int C = E::kVec, M = G / kWave;
+    const int wave = G > kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave) : 0;
+    const double tiny = sum * 0x1p-80;
     // the part (vector, wave) that holds the level, and what comes before it
     int part = -1, some = 0;
     double before = 0;
-#pragma unroll
-    for (int i = 0; i < NV * M; i++) {
-        if (part < 0 && before + sums[i] > level) part = i;
-        if (part < 0) before += sums[i];
-        if (sums[i] > kTiny) some = i;
+#pragma unroll 1
+    for (int i = 0; i < nv * M; i++) {
+        if (before + sums[i] > level) {
+            part = i;
+            break;
+        }
+        before += sums[i];
+        if (sums[i] > tiny) some = i;
     }
     if (part < 0) {
         part = some;
         before = 0;
         level = INFINITY;
     }
-    const int kk = NV == 1 ? 0 : __builtin_amdgcn_readfirstlane(part / M), ww = part - kk * M;   // NV > 1 has one row in a wave
+    part = __builtin_amdgcn_readfirstlane(part);
+    const int k = part / M, at_wave = part - k * M;
     int column = 0;
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-        if (NV > 1 && kk != k) continue;
-        const double upto = running_sum<W>(s[k], lane);
-        const int self = (int)(threadIdx.x & (kWave - 1));
-        const uint64_t group = W == 64 ? ~0ull : ((1ull << W) - 1) << (self & ~(W - 1));
-        const uint64_t hits = __ballot(s[k] > 0 && before + upto > level) & group, any = __ballot(s[k] > kTiny) & group;
-        const int first = hits ? __ffsll((unsigned long long)hits) - 1 : any ? 63 - __clzll((long long)any) : self;
-        // every lane walks its own vector; the chosen lane's answer counts
-        typename Tile<E, RULES, NV, C>::Y y[C];
-        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
-        double acc = before + (upto - s[k]);
-        int at = -1, last = 0;
-#pragma unroll
-        for (int j = 0; j < C; j++) {
-            const double e = weight((double)y[j], base, k2);
-            acc += e;
-            if (e > kTiny) {
-                last = j;
-                if (at < 0 && acc > level) at = j;
-            }
-        }
-        if (at < 0) at = last;
-        if (W > 1) at = __shfl(at, first);
-        column = (k * G + (G > kWave ? ww * kWave : 0) + (first & (W - 1))) * C + at;
+    if (wave == at_wave) {
+        Vector<E, C> v;
+        v.load(w, x, p.at + k * p.step, p.width);
+        double s = 0, e[C];
+        with_y<E, RULES, C>(w, p, k, v, [&](const auto* y) { s = weigh<C>(y, base, c, e); });
+        column = (k * G + at_wave * kWave) * C + walk<kWave, C>(e, s, before, level, tiny);
+        if (G > kWave && (threadIdx.x & (kWave - 1)) == 0) *lds_at = column;
     }
     if (G > kWave) {
-        if (wave == ww && lane == 0) *lds_at = column;
         __syncthreads();
         column = *lds_at;
+        __syncthreads();
     }
     return column;
 }
 
-// The first column of the row where the tile holds m, or `none`.
-template <typename E, bool RULES, int G, int NV, int C>
-__device__ inline int64_t first_of(const Tile<E, RULES, NV, C>& tile, const Row& w, double m, int64_t v0, int step, int64_t width, const uint32_t* counts,
-                                   long long* lds) {
-    long long at = width;
-#pragma unroll
-    for (int k = NV - 1; k >= 0; k--) {
-        typename Tile<E, RULES, NV, C>::Y y[C];
-        tile.get(k, w, v0 + k * step, width, counts ? counts + k * step : nullptr, y);
-#pragma unroll
-        for (int j = C - 1; j >= 0; j--)
-            if ((double)y[j] == m) at = v0 + k * step + j;
-    }
-    return group_reduce<G>(at, Min<long long>(), lds);
-}
-
-__device__ inline float log_prob_of(double y, double m, double k2, double sum) { return (float)(((y - m) * k2 - log2_double(sum)) * kLn2); }
-
-// A row in G lanes' registers: rows of at most G * C * NV columns, kBlock / G of them per workgroup.
-template <typename E, bool RULES, int G, int NV, int C>
-__global__ void __launch_bounds__(kBlock) sample_rows_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
-                                                             int32_t* actions, float* log_prob) {
-    constexpr int per = kBlock / G, cap = G * C * NV, step = G * C;
-    __shared__ __align__(16) uint32_t counts[RULES ? per * cap : 4];
-    __shared__ double lds[NV * (kBlock / kWave)];
-    __shared__ long long lds_first[kBlock / kWave];
+// Rows of one strip: by a wave each (G = 64), or a workgroup.
+template <typename E, bool RULES, int G>
+__global__ void __launch_bounds__(kBlock) sample_strips_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
+                                                               int nv, bool half, int32_t* actions, float* log_prob) {
+    constexpr int C = E::kVec, per = kBlock / G, M = G / kWave;
+    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ double lds[kBlock / kWave];
+    __shared__ double sums[per][kTile * M];
     __shared__ int lds_at;
-    const int lane = (int)threadIdx.x & (G - 1);
-    const int group = G >= kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : (int)threadIdx.x / G;
+    const int cap = G * C * nv;
+    const int lane = (int)threadIdx.x & (G - 1), group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : 0;
+    const bool hist = RULES && r.hist;
+    const Counts counts{hist ? words : nullptr, cap, per * cap, half, true};
     for (int64_t band = blockIdx.x; band * per < rows; band += gridDim.x) {
-        if (RULES && r.hist) count_ids(r, band * per, per, rows, width, 0, cap, counts);
         const int64_t own = band * per + group;
-        const int64_t b = own < rows ? own : rows - 1;   // lanes without a row follow the last one: every exchange has all its lanes
+        const int64_t b = own < rows ? own : rows - 1;
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const int64_t v0 = lane * C;
-        const uint32_t* mine = RULES && r.hist ? counts + group * cap : nullptr;
-        const uint32_t* here = mine ? mine + v0 : nullptr;
-        Tile<E, RULES, NV, C> tile;
-        tile.load(x, v0, step, width);
-        const double u = row_uniform(keys, b);
-        const double k2 = kLog2e / w.temp;
-        double s[NV], m, sum;
-        bool bad;
-        sum_tile<E, RULES, G, NV, C>(tile, w, v0, step, width, here, k2, lds, s, &m, &sum, &bad);
-        const double base = m > -INFINITY && m < INFINITY ? m : 0.0;
-        int64_t at = locate<E, RULES, G, NV, C>(tile, w, v0, step, width, here, s, base, k2, u * sum, lds, &lds_at);
-        if (G > kWave ? w.greedy : __any(w.greedy)) {   // the same for all lanes that exchange
-            const int64_t first = first_of<E, RULES, G, NV, C>(tile, w, m, v0, step, width, here, lds_first);
-            if (w.greedy) at = first;
+        const Place p{lane * C, width, G * C, group * cap + lane * C, counts};
+        Vector<E, C> v;
+        v.load(w, x, p.at, width);
+        if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
+        const Scale c = scale_of(w);
+        long long first = 0;
+        const Mass mass = sum_strip<E, RULES, G>(x, v, w, p, nv, c, lds, &first);
+        int64_t at = first;
+        if (!w.greedy && !mass.bad && mass.base > -INFINITY) {   // the group's lanes alike
+            strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums[group]);
+            at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums[group], &lds_at);
         }
-        if (lane == 0 && own < rows) {
-            float lp = bad ? NAN : -INFINITY;
-            if (bad || m == -INFINITY) at = -1;
-            else lp = log_prob_of(ruled(w, (float)x[at], mine ? mine[at] : 0u, true, at), m, k2, sum);
-            actions[b] = (int32_t)at;
-            log_prob[b] = lp;
-        }
+        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob);
     }
 }
 
-// Wider rows: one workgroup per tile leaves the tile's greatest y, the sum of its weights against that, and where it is first; then one
-// workgroup per row joins them, finds the tile that the level falls into and goes through that tile once more.
+// Wider rows: one workgroup per strip leaves the sum of the strip's weights, against which base, and where in a greedy row that base (its
+// greatest y) is first; then one workgroup per row joins them, finds the strip that the level falls into and goes through that strip once more.
 struct Part {
-    double m, s;
+    double base, sum;   // an empty part: -inf, 0;  one with a NaN or +inf: sum NaN
     long long first;
 };
 
-template <typename E, bool RULES, int NV>
-__global__ void __launch_bounds__(kBlock) sample_parts_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int64_t cuts,
-                                                              Part* parts) {
-    constexpr int C = E::kVec, cap = kBlock * C * NV, step = kBlock * C;
-    __shared__ __align__(16) uint32_t counts[RULES ? cap : 4];
+template <typename E, bool RULES>
+__global__ void __launch_bounds__(kBlock) sample_parts_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int nv, bool half,
+                                                              int64_t cuts, Part* parts) {
+    constexpr int C = E::kVec;
+    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
     __shared__ double lds[kBlock / kWave];
-    __shared__ long long lds_first[kBlock / kWave];
-    for (int64_t i = blockIdx.x; i < rows * cuts; i += gridDim.x) {
-        const int64_t b = i / cuts, lo = (i - b * cuts) * cap;
-        const int64_t v0 = lo + threadIdx.x * C;
-        Tile<E, RULES, NV, C> tile;
-        tile.load(x0 + b * stride, v0, step, width);
-        if (RULES && r.hist) count_ids(r, b, 1, rows, width, lo, cap, counts);
-        const uint32_t* here = RULES && r.hist ? counts + threadIdx.x * C : nullptr;
+    const int cap = kBlock * C * nv, place = (int)threadIdx.x * C;
+    const bool hist = RULES && r.hist;
+    const Counts counts{hist ? words : nullptr, cap, cap, half, true};
+    const int64_t lo = (int64_t)blockIdx.x * cap;
+    for (int64_t b = blockIdx.y; b < rows; b += gridDim.y) {
         const Row w = row_of<RULES>(r, b);
-        double s[NV], m, sum;
-        bool bad;
-        sum_tile<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, kLog2e / w.temp, lds, s, &m, &sum, &bad);
-        const int64_t first = w.greedy ? first_of<E, RULES, kBlock, NV, C>(tile, w, m, v0, step, width, here, lds_first) : 0;
-        if (threadIdx.x == 0) parts[i] = Part{m, bad ? (double)NAN : m == -INFINITY ? 0.0 : sum, first};
+        const Place p{lo + place, width, kBlock * C, place, counts};
+        const typename E::T* x = x0 + b * stride;
+        Vector<E, C> v;
+        v.load(w, x, p.at, width);
+        if (hist) count_ids(r, b, 1, rows, width, lo, counts);
+        long long first = 0;
+        const Mass mass = sum_strip<E, RULES, kBlock>(x, v, w, p, nv, scale_of(w), lds, &first);
+        if (threadIdx.x == 0) parts[b * cuts + blockIdx.x] = Part{mass.base, mass.bad ? (double)NAN : mass.base == -INFINITY ? 0.0 : mass.sum, first};
     }
 }
 
-template <typename E, bool RULES, int NV>
-__global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
-                                                             int64_t cuts, const Part* parts, int32_t* actions, float* log_prob) {
-    constexpr int C = E::kVec, cap = kBlock * C * NV, step = kBlock * C;
-    __shared__ __align__(16) uint32_t counts[RULES ? cap : 4];
-    __shared__ double lds[NV * (kBlock / kWave)];
-    __shared__ long long lds_first[kBlock / kWave];
+// Every wave of a row's workgroup finds the strip by itself, 64 parts at a time: that takes no barrier.
+template <typename E, bool RULES>
+__global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys, int nv,
+                                                             bool half, int64_t cuts, const Part* parts, int32_t* actions, float* log_prob) {
+    constexpr int C = E::kVec;
+    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ double sums[kTile * (kBlock / kWave)];
     __shared__ int lds_at;
-    __shared__ double before_part;
-    __shared__ int the_part;
+    const int cap = kBlock * C * nv, place = (int)threadIdx.x * C, lane = (int)threadIdx.x & (kWave - 1);
+    const bool hist = RULES && r.hist;
+    const Counts counts{hist ? words : nullptr, cap, cap, half, true};
+    double* const none = nullptr;
     for (int64_t b = blockIdx.x; b < rows; b += gridDim.x) {
-        const Part* p = parts + b * cuts;
+        const Part* parts_b = parts + b * cuts;
         const Row w = row_of<RULES>(r, b);
-        const double k2 = kLog2e / w.temp;
+        const Scale scale = scale_of(w);
+        const typename E::T* x = x0 + b * stride;
+        const double u = row_uniform(keys, b);
         double m = -INFINITY;
         int bad = 0;
-        for (int64_t c = threadIdx.x; c < cuts; c += kBlock) {
-            m = p[c].m > m ? p[c].m : m;
-            bad |= p[c].s != p[c].s;
+        for (int64_t c = lane; c < cuts; c += kWave) {
+            m = parts_b[c].base > m ? parts_b[c].base : m;
+            bad |= parts_b[c].sum != parts_b[c].sum;
         }
-        m = group_reduce<kBlock>(m, Max<double>(), lds);
-        bad = group_reduce<kBlock>(bad, Max<int>(), (int*)lds);
-        if (bad || m == -INFINITY) {   // the same for the whole workgroup
-            if (threadIdx.x == 0) {
-                actions[b] = -1;
-                log_prob[b] = bad ? NAN : -INFINITY;
-            }
-            continue;
-        }
-        auto share = [&](int64_t c) { return c < cuts && p[c].s > 0 ? p[c].s * weight(p[c].m, m, k2) : 0.0; };
+        m = group_reduce<kWave>(m, Max<double>(), none);
+        bad = group_reduce<kWave>(bad, Max<int>(), (int*)none);
+        const bool any = !bad && m > -INFINITY;   // the same for the whole workgroup, as is what hangs on it
+        // a part's sum against m
+        auto share = [&](int64_t c) { return c < cuts && parts_b[c].sum > 0 ? parts_b[c].sum * weight(parts_b[c].base - m, scale) : 0.0; };
         double sum = 0;
         long long first = width;
-        for (int64_t c = threadIdx.x; c < cuts; c += kBlock) {
-            sum += share(c);
-            if (p[c].m == m && p[c].first < first) first = p[c].first;
-        }
-        sum = group_reduce<kBlock>(sum, Sum<double>(), lds);
-        int64_t at;
-        if (w.greedy) {
-            at = group_reduce<kBlock>(first, Min<long long>(), lds_first);
-            if (RULES && r.hist) count_ids(r, b, 1, rows, width, at / cap * cap, cap, counts);
-        } else {
-            const double level = row_uniform(keys, b) * sum;
-            if (threadIdx.x == 0) the_part = -1;
-            double run = 0;
-            int last = 0;   // the last part with any weight, should rounding leave the level above all sums
-            for (int64_t c0 = 0; c0 < cuts; c0 += kBlock) {
-                const int64_t c = c0 + threadIdx.x;
-                const double e = share(c);
-                const int lane = (int)threadIdx.x & (kWave - 1), wave = (int)threadIdx.x / kWave;
-                const double upto = running_sum<kWave>(e, lane);
-                __syncthreads();
-                if (lane == kWave - 1) lds[wave] = upto;
-                __syncthreads();
-                double front = run;
-                for (int i = 0; i < kBlock / kWave; i++) {
-                    if (i < wave) front += lds[i];
-                    run += lds[i];
-                }
-                const long long hit = e > 0 && front + upto > level ? (long long)c : (long long)cuts;
-                const long long least = group_reduce<kBlock>(hit, Min<long long>(), lds_first);
-                if (least < cuts) {
-                    if (c == least) {
-                        the_part = (int)c;
-                        before_part = front + (upto - e);
-                    }
-                    break;
-                }
-                const long long most = group_reduce<kBlock>(e > 0 ? (long long)c : -1ll, Max<long long>(), lds_first);
-                if (most >= 0) last = (int)most;
+        if (any)
+            for (int64_t c = lane; c < cuts; c += kWave) {
+                sum += share(c);
+                if (parts_b[c].base == m && parts_b[c].first < first) first = parts_b[c].first;
             }
-            __syncthreads();
-            const bool over = the_part < 0;
-            const int c = over ? last : the_part;
-            const double top = p[c].m;
-            const double target = over ? INFINITY : (level - before_part) / weight(top, m, k2);
-            const int64_t lo = (int64_t)c * cap, v0 = lo + threadIdx.x * C;
-            Tile<E, RULES, NV, C> tile;
-            tile.load(x0 + b * stride, v0, step, width);
-            if (RULES && r.hist) count_ids(r, b, 1, rows, width, lo, cap, counts);
-            const uint32_t* here = RULES && r.hist ? counts + threadIdx.x * C : nullptr;
-            double s[NV], tile_m, tile_sum;
-            bool tile_bad;
-            sum_tile<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, k2, lds, s, &tile_m, &tile_sum, &tile_bad);
-            at = lo + locate<E, RULES, kBlock, NV, C>(tile, w, v0, step, width, here, s, top, k2, target, lds, &lds_at);
+        const Mass mass{m, group_reduce<kWave>(sum, Sum<double>(), none), bad != 0};
+        int64_t at = 0;
+        if (any && w.greedy) {
+            at = group_reduce<kWave>(first, Min<long long>(), (long long*)none);
+            if (hist) count_ids(r, b, 1, rows, width, at / cap * cap, counts);
+        } else if (any) {
+            const double level = u * mass.sum, tiny = mass.sum * 0x1p-80;
+            int64_t part = -1, last = 0;   // last: the last part with any weight, should rounding leave the level above all sums
+            double run = 0, before = 0;
+            for (int64_t c0 = 0; c0 < cuts && part < 0; c0 += kWave) {
+                const double e = share(c0 + lane);
+                const double upto = running_sum<kWave>(e, lane);
+                const uint64_t hits = __ballot(e > 0 && run + upto > level), some = __ballot(e > tiny);
+                if (hits) {
+                    const int at_lane = __ffsll((unsigned long long)hits) - 1;
+                    part = c0 + at_lane;
+                    before = run + __shfl(upto - e, at_lane);
+                } else if (some) {
+                    last = c0 + 63 - __clzll((long long)some);
+                }
+                run += __shfl(upto, kWave - 1);
+            }
+            const int64_t c = part < 0 ? last : part;
+            const double base = parts_b[c].base;
+            const double target = part < 0 ? INFINITY : (level - before) / weight(base - m, scale);
+            const int64_t lo = c * cap;
+            const Place p{lo + place, width, kBlock * C, place, counts};
+            Vector<E, C> v;
+            v.load(w, x, p.at, width);
+            if (hist) count_ids(r, b, 1, rows, width, lo, counts);
+            strip_sums<E, RULES, kBlock>(x, v, w, p, nv, scale, base, sums);
+            at = lo + locate<E, RULES, kBlock>(x, w, p, nv, scale, base, parts_b[c].sum, target, sums, &lds_at);
         }
-        if (threadIdx.x == 0) {
-            const uint32_t n = RULES && r.hist ? counts[at % cap] : 0u;
-            actions[b] = (int32_t)at;
-            log_prob[b] = log_prob_of(ruled(w, (float)x0[b * stride + at], n, true, at), m, k2, sum);
-        }
+        if (threadIdx.x == 0) answer<E>(w, x, mass, at, any && hist ? counts.at((int)(at % cap)) : 0u, scale, b, actions, log_prob);
         __syncthreads();
     }
 }
 
-// Tiles along a row of the wide form: NV = 4 vectors a lane where that still makes enough workgroups, else 1.
+// Vectors a lane in a strip, at most: what the counts' LDS holds.  (Without a history there could be more; of 8 or 16 the parts take 5 us less of
+// 512 x 131,072 bf16, and the join, which goes through one strip once more, 10 to 15 us more.)
+int strip_vectors(const Rules& r) { return r.hist && !half_counts(r) ? kTile / 2 : kTile; }
 int64_t cuts_of(int vec, int nv, int64_t width) {
     const int64_t cap = (int64_t)kBlock * vec * nv;
     return (width + cap - 1) / cap;
 }
-bool is_wide(int vec, int64_t width) { return width > (int64_t)kBlock * vec * 4; }
-int wide_nv(int vec, int64_t rows, int64_t width) { return rows * cuts_of(vec, 4, width) < 1024 ? 1 : 4; }
-
-size_t parts_bytes(int vec, int64_t rows, int64_t width) {
-    if (!is_wide(vec, width)) return 0;
-    return sizeof(Part) * (size_t)rows * (size_t)cuts_of(vec, wide_nv(vec, rows, width), width);
+// The wide form's: as many as still make workgroups enough to fill the chip.
+int wide_nv(int vec, int most, int64_t rows, int64_t width) {
+    int nv = most;
+    while (nv > 1 && rows * cuts_of(vec, nv, width) < 1024) nv /= 2;
+    return nv;
 }
 
-template <typename E, bool RULES, int G, int NV, int C>
-void launch_rows(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const Keys& k, int32_t* actions, float* log_prob, hipStream_t s) {
-    constexpr int per = kBlock / G;
-    hipLaunchKernelGGL((sample_rows_kernel<E, RULES, G, NV, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, (const typename E::T*)x, rows,
-                       width, stride, r, k, actions, log_prob);
-}
-
-template <typename E, bool RULES, int NV>
-void launch_wide(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const Keys& k, int32_t* actions, float* log_prob, void* ws,
-                 hipStream_t s) {
-    const int64_t cuts = cuts_of(E::kVec, NV, width);
-    hipLaunchKernelGGL((sample_parts_kernel<E, RULES, NV>), dim3(grid_for(rows * cuts)), dim3(kBlock), 0, s, (const typename E::T*)x, rows, width, stride, r,
-                       cuts, (Part*)ws);
-    hipLaunchKernelGGL((sample_join_kernel<E, RULES, NV>), dim3(grid_for(rows)), dim3(kBlock), 0, s, (const typename E::T*)x, rows, width, stride, r, k, cuts,
-                       (const Part*)ws, actions, log_prob);
+// For any type and rules.
+size_t parts_bytes(int64_t rows, int64_t width) {
+    size_t most = 0;
+    for (const int vec : {F32::kVec, F16::kVec})
+        for (const int nv : {kTile / 2, kTile}) {
+            const size_t bytes = sizeof(Part) * (size_t)rows * (size_t)cuts_of(vec, wide_nv(vec, nv, rows, width), width);
+            if (width > (int64_t)kBlock * vec * nv && bytes > most) most = bytes;
+        }
+    return most;
 }
 
 template <typename E, bool RULES>
-void launch(const void* x, int64_t rows, int64_t width, int64_t stride, const Rules& r, const Keys& k, int32_t* actions, float* log_prob, void* ws,
-            hipStream_t s) {
-    constexpr int v = E::kVec;
-    // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each
-    if (width <= 2) launch_rows<E, RULES, 1, 1, 2>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 4) launch_rows<E, RULES, 1, 1, 4>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= v) launch_rows<E, RULES, 1, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 2 * v) launch_rows<E, RULES, 2, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 4 * v) launch_rows<E, RULES, 4, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 8 * v) launch_rows<E, RULES, 8, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 16 * v) launch_rows<E, RULES, 16, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 64 * v) launch_rows<E, RULES, 64, 1, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (width <= 64 * v * 4) launch_rows<E, RULES, 64, 4, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (!is_wide(v, width)) launch_rows<E, RULES, kBlock, 4, v>(x, rows, width, stride, r, k, actions, log_prob, s);
-    else if (wide_nv(v, rows, width) == 1) launch_wide<E, RULES, 1>(x, rows, width, stride, r, k, actions, log_prob, ws, s);
-    else launch_wide<E, RULES, 4>(x, rows, width, stride, r, k, actions, log_prob, ws, s);
-}
+struct Launch {
+    const typename E::T* x;
+    int64_t rows, width, stride;
+    const Rules& r;
+    const Keys& k;
+    int32_t* actions;
+    float* log_prob;
+    void* ws;
+    hipStream_t s;
+
+    template <int G, int C>
+    void vectors() const {
+        constexpr int per = kBlock / G;
+        hipLaunchKernelGGL((sample_vectors_kernel<E, RULES, G, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r, k,
+                           actions, log_prob);
+    }
+    template <int G>
+    void strips(int nv) const {
+        constexpr int per = kBlock / G;
+        hipLaunchKernelGGL((sample_strips_kernel<E, RULES, G>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r, k, nv,
+                           half_counts(r), actions, log_prob);
+    }
+    void wide(int nv) const {
+        const int64_t cuts = cuts_of(E::kVec, nv, width);
+        hipLaunchKernelGGL((sample_parts_kernel<E, RULES>), dim3((unsigned)cuts, grid_for(rows, 65535)), dim3(kBlock), 0, s, x, rows, width, stride, r, nv, half_counts(r), cuts,
+                           (Part*)ws);
+        hipLaunchKernelGGL((sample_join_kernel<E, RULES>), dim3(grid_for(rows)), dim3(kBlock), 0, s, x, rows, width, stride, r, k, nv, half_counts(r), cuts,
+                           (const Part*)ws, actions, log_prob);
+    }
+    void operator()() const {
+        constexpr int v = E::kVec;
+        const int most = strip_vectors(r);
+        const auto need = [&](int g) { return (int)((width + g * v - 1) / (g * v)); };   // vectors a lane
+        // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then strips
+        if (width <= 2) vectors<1, 2>();
+        else if (width <= 4) vectors<1, 4>();
+        else if (width <= v) vectors<1, v>();
+        else if (width <= 2 * v) vectors<2, v>();
+        else if (width <= 4 * v) vectors<4, v>();
+        else if (width <= 8 * v) vectors<8, v>();
+        else if (width <= 16 * v) vectors<16, v>();
+        else if (width <= 32 * v) vectors<32, v>();
+        else if (width <= 64 * v) vectors<64, v>();
+        else if (width <= 64 * v * most) strips<64>(need(64));
+        else if (width <= (int64_t)kBlock * v * most) strips<kBlock>(need(kBlock));
+        else wide(wide_nv(v, most, rows, width));
+    }
+};
 
 }  // namespace
 }  // namespace policy
@@ -400,8 +558,7 @@ extern "C" {
 
 size_t gymhip_sample_workspace_bytes(int64_t rows, int64_t width) {
     if (rows <= 0 || width <= 0 || width > GYMHIP_POLICY_MAX_WIDTH) return 0;
-    const size_t a = parts_bytes(F32::kVec, rows, width), b = parts_bytes(F16::kVec, rows, width);
-    return a > b ? a : b;
+    return parts_bytes(rows, width);
 }
 
 int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
@@ -417,7 +574,7 @@ int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t wi
     return with_type(type, [&](auto e) {
         using E = decltype(e);
         with_bool(!r.plain(), [&](auto ruled_) {
-            launch<E, decltype(ruled_)::value>(logits, rows, width, stride, r, k, actions, log_prob, workspace, (hipStream_t)stream);
+            Launch<E, decltype(ruled_)::value>{(const typename E::T*)logits, rows, width, stride, r, k, actions, log_prob, workspace, (hipStream_t)stream}();
         });
     });
 }
