@@ -16,7 +16,6 @@ gym_amd.vec_env calls them from VecLogitActions (step(logits)) and VecObservatio
 """
 from __future__ import annotations
 
-import copy
 import ctypes as C
 from typing import NamedTuple
 
@@ -34,27 +33,32 @@ class ActionSample(NamedTuple):
     log_prob: torch.Tensor
 
 
-def _raw_stream(device):
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(device.index) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _on_device(fn):
-    """Kernels go to the current device: make the first argument's device current where it is not."""
-    def call(x, *args):
-        if x.device.index != torch.cuda.current_device():
-            with torch.cuda.device(x.device):
-                return fn(x, *args)
-        return fn(x, *args)
-    return call
+def _call(name, x, *args):
+    """The entry point on x's device and its current stream."""
+    index = x.device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(_lib or _load(), name)(*args, _raw_stream(index))
+    else:   # kernels go to the current device
+        with torch.cuda.device(index):
+            rc = getattr(_lib or _load(), name)(*args, _raw_stream(index))
+    if rc:
+        L.check(rc, name)
 
 
-def _checked(rules):
-    if rules is not None and not isinstance(rules, LogitRules):
-        raise ValueError("rules must be a LogitRules")
+_lib = None
 
 
-def _matrix(x, what):
+def _load():
+    global _lib
+    _lib = L.load()
+    return _lib
+
+
+def _ready(x, rules=None, what="logits"):
+    """x where it is a matrix the kernels take, its rows in order and its columns adjacent (rows may be apart, or all the same one); else a copy."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{what} must be a 2-D tensor [rows, width]")
     if x.dtype not in _TYPES:
@@ -63,11 +67,19 @@ def _matrix(x, what):
         raise L.GymhipError(f"{what} is on {x.device}: the policy kernels run on the GPU and have no CPU fallback")
     if x.shape[1] > L.POLICY_MAX_WIDTH:
         raise ValueError(f"{what}: at most 2^24 columns, got {x.shape[1]}")
+    if rules is not None and not isinstance(rules, LogitRules):
+        raise ValueError("rules must be a LogitRules")
+    return _rowwise(x)
 
 
 def _rowwise(x):
-    """x itself where its columns are adjacent and its rows lie in order (rows may be apart, or all the same one), else a copy."""
-    return x if (x.stride(1) == 1 or x.shape[1] == 1) and x.stride(0) >= 0 else x.contiguous()
+    row, column = x.stride()
+    return x if (column == 1 or x.shape[1] == 1) and row >= 0 else x.contiguous()
+
+
+def _empty_like(x):
+    """A contiguous matrix of x's shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _side(t, what, device, dtypes, shapes):
@@ -80,6 +92,9 @@ def _side(t, what, device, dtypes, shapes):
     if tuple(t.shape) not in shapes:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {' or '.join(str(s) for s in shapes)}")
     return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+_RULES_SIZE = C.sizeof(L.LogitRules)
 
 
 class LogitRules:
@@ -122,8 +137,7 @@ class LogitRules:
     def _bind(self, logits):
         """(C struct, tensors it points into) for these logits; checks every shape, type and device."""
         rows, width = logits.shape
-        dev, c, keep = logits.device, L.LogitRules(), []
-        c.struct_size = C.sizeof(L.LogitRules)
+        dev, c, keep = logits.device, L.LogitRules(_RULES_SIZE), []
         if self.mask is not None:
             words = (width + 31) // 32
             m = self.mask
@@ -180,100 +194,87 @@ def pack_action_mask(allowed: torch.Tensor) -> torch.Tensor:
     return (bits << torch.arange(32, device=allowed.device)).sum(2).to(torch.int32)   # the low 32 bits, bit 31 as the sign
 
 
-def _keys(rows_n, device, seed, step, rows):
+def _keys(n, device, seed, step, rows):
     """(C struct, tensors it points into)"""
-    k, keep = L.RandomKeys(), []
-    k.struct_size = C.sizeof(L.RandomKeys)
-    k.seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+    if type(step) is int and type(rows) is int:
+        return L.RandomKeys(_KEYS_SIZE, 0, seed & _U64, rows, step, None, None), ()
+    k, keep = L.RandomKeys(_KEYS_SIZE, 0, int(seed) & _U64), []
     if isinstance(rows, torch.Tensor):
-        t = _side(rows, "rows", device, (torch.int64,), ((rows_n,),))
+        t = _side(rows, "rows", device, (torch.int64,), ((n,),))
         k.rows = t.data_ptr()
         keep.append(t)
     else:
         k.row = int(rows)
     if isinstance(step, torch.Tensor):
-        t = _side(step, "step", device, (torch.int64,), ((), (1,), (rows_n,)))
-        k.steps, k.steps_per_row = t.data_ptr(), int(t.dim() == 1 and t.shape[0] == rows_n)
+        t = _side(step, "step", device, (torch.int64,), ((), (1,), (n,)))
+        k.steps, k.steps_per_row = t.data_ptr(), int(t.dim() == 1 and t.shape[0] == n)
         keep.append(t)
     else:
         k.step = int(step)
     return k, keep
 
 
-def _bound(rules, logits):
-    if rules is None:
-        return None, None, []
-    c, keep = rules._bind(logits)
-    return C.byref(c), c, keep
+_KEYS_SIZE, _U64 = C.sizeof(L.RandomKeys), 0xFFFFFFFFFFFFFFFF
 
 
-@_on_device
-def _process(x, rules, out):
-    ref, _, keep = _bound(rules, x)
-    L.check(L.load().gymhip_process_logits(x.data_ptr(), _TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), ref, out.data_ptr(), out.stride(0),
-                                           _raw_stream(x.device)), "gymhip_process_logits")
-    return out
+def _save(ctx, rules, bound, *tensors):
+    """For the backward pass: the tensors (its pointers are taken from what comes back: hooks may move saved tensors), the C struct of the rules with
+    what it points into, and the rules' tensors among the saved ones, so that changing one in place before it raises."""
+    ctx.bound = bound
+    ctx.save_for_backward(*tensors, *rules._tensors()) if rules is not None else ctx.save_for_backward(*tensors)
 
 
-@_on_device
-def _process_backward(x, rules, grad):
-    ref, _, keep = _bound(rules, x)
-    grad = _rowwise(grad)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    L.check(L.load().gymhip_process_logits_backward(x.data_ptr(), _TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), ref, grad.data_ptr(), grad.stride(0),
-                                                    out.data_ptr(), out.stride(0), _raw_stream(x.device)), "gymhip_process_logits_backward")
-    return out
+def _bind(rules, x):
+    """None, or (C struct, the tensors it points into)"""
+    return None if rules is None else rules._bind(x)
 
 
-def _save(ctx, rules, *tensors):
-    """Tensors and rules for the backward pass; the rules' tensors are saved too, so that changing one in place before it raises."""
-    ctx.save_for_backward(*tensors, *(rules._tensors() if rules is not None else ()))
-    ctx.rules = copy.copy(rules)
+def _head(x, bound):
+    """(logits, type, rows, width, stride, rules) of a C call"""
+    n, width = x.shape
+    return x.data_ptr(), _TYPES[x.dtype], n, width, x.stride(0), None if bound is None else C.byref(bound[0])
+
+
+def _once():
+    """The gradients' own kernels have no gradient: under create_graph autograd would take them for constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the policy operators are differentiable once: create_graph is not available")
 
 
 class _Process(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rules):
         x = _rowwise(logits)
-        _save(ctx, rules, x)
-        return _process(x, rules, torch.empty(x.shape, dtype=x.dtype, device=x.device))
+        bound = _bind(rules, x)
+        _save(ctx, rules, bound, x)
+        out = _empty_like(x)
+        _call("gymhip_process_logits", x, *_head(x, bound), out.data_ptr(), out.stride(0))
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        return _process_backward(ctx.saved_tensors[0], ctx.rules, grad), None
+        _once()
+        x, grad = _rowwise(ctx.saved_tensors[0]), _rowwise(grad)
+        out = _empty_like(x)
+        _call("gymhip_process_logits_backward", x, *_head(x, ctx.bound), grad.data_ptr(), grad.stride(0), out.data_ptr(), out.stride(0))
+        return out, None
 
 
 def process_logits(logits: torch.Tensor, rules: LogitRules | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """z (LogitRules) of logits [rows, width], rounded once to their type.  Differentiable in the logits.  `out` (not under autograd) may
     be the logits themselves, or memory that does not touch them."""
-    _matrix(logits, "logits")
-    _checked(rules)
+    x = _ready(logits, rules)
     if out is None:
-        return _Process.apply(logits, rules) if logits.requires_grad and torch.is_grad_enabled() else _process(
-            _rowwise(logits), rules, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
-    if torch.is_grad_enabled() and (logits.requires_grad or out.requires_grad):
+        if logits.requires_grad and torch.is_grad_enabled():
+            return _Process.apply(logits, rules)
+        out = _empty_like(x)
+    elif torch.is_grad_enabled() and (logits.requires_grad or out.requires_grad):
         raise ValueError("out= is not available under autograd")
-    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (out.stride(1) != 1 and out.shape[1] > 1):
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (out.stride(1) != 1 and out.shape[1] > 1):
         raise ValueError("out must have the logits' shape, type and device, and adjacent columns")
-    return _process(_rowwise(logits), rules, out)
-
-
-@_on_device
-def _sample(x, rules, seed, step, rows, actions, log_prob):
-    lib = L.load()
-    n, width = x.shape
-    ref, _, keep = _bound(rules, x)
-    k, keep2 = _keys(n, x.device, seed, step, rows)
-    nbytes = lib.gymhip_sample_workspace_bytes(n, width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    if actions is None:
-        actions = torch.empty(n, dtype=torch.int32, device=x.device)
-    if log_prob is None:
-        log_prob = torch.empty(n, dtype=torch.float32, device=x.device)
-    L.check(lib.gymhip_sample_actions(x.data_ptr(), _TYPES[x.dtype], n, width, x.stride(0), ref, C.byref(k), actions.data_ptr(), log_prob.data_ptr(),
-                                      ws.data_ptr() if nbytes else None, nbytes, _raw_stream(x.device)), "gymhip_sample_actions")
-    return ActionSample(actions, log_prob)
+    bound = _bind(rules, x)
+    _call("gymhip_process_logits", x, *_head(x, bound), out.data_ptr(), out.stride(0))
+    return out
 
 
 def sample_actions(logits: torch.Tensor, rules: LogitRules | None = None, *, seed: int, step=0, rows=0, out: ActionSample | None = None) -> ActionSample:
@@ -283,44 +284,36 @@ def sample_actions(logits: torch.Tensor, rules: LogitRules | None = None, *, see
     between replays of a captured graph) or int64 [rows].  Keys and steps count modulo 2^48.
 
     A row with nothing allowed gives action -1 and log-probability -inf, a row with a NaN or +inf among its allowed z -1 and NaN."""
-    _matrix(logits, "logits")
-    _checked(rules)
-    a = p = None
-    if out is not None:
-        a, p = out
-        _side(a, "out.actions", logits.device, (torch.int32,), ((logits.shape[0],),))
-        _side(p, "out.log_prob", logits.device, (torch.float32,), ((logits.shape[0],),))
-        if not (a.is_contiguous() and p.is_contiguous()):
-            raise ValueError("out tensors must be contiguous")
-    return _sample(_rowwise(logits.detach()), rules, seed, step, rows, a, p)
-
-
-@_on_device
-def _score(x, rules, actions):
-    lib = L.load()
+    x = _ready(logits, rules)
     n, width = x.shape
-    ref, _, keep = _bound(rules, x)
-    nbytes = lib.gymhip_action_log_prob_workspace_bytes(n, width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    lp = torch.empty(n, dtype=torch.float32, device=x.device)
-    ent = torch.empty(n, dtype=torch.float32, device=x.device)
-    lse = torch.empty(n, 2, dtype=torch.float64, device=x.device)
-    L.check(lib.gymhip_action_log_prob(x.data_ptr(), _TYPES[x.dtype], n, width, x.stride(0), ref, actions.data_ptr(), _INTS[actions.dtype], lp.data_ptr(),
-                                       ent.data_ptr(), lse.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, _raw_stream(x.device)), "gymhip_action_log_prob")
-    return lp, ent, lse
+    device = x.device
+    if out is None:
+        actions, log_prob = torch.empty(n, dtype=torch.int32, device=device), torch.empty(n, dtype=torch.float32, device=device)
+    else:
+        actions, log_prob = out
+        _side(actions, "out.actions", device, (torch.int32,), ((n,),))
+        _side(log_prob, "out.log_prob", device, (torch.float32,), ((n,),))
+        if not (actions.is_contiguous() and log_prob.is_contiguous()):
+            raise ValueError("out tensors must be contiguous")
+    bound = _bind(rules, x)
+    k, keep_keys = _keys(n, device, seed, step, rows)
+    nbytes = (_lib or _load()).gymhip_sample_workspace_bytes(n, width)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _call("gymhip_sample_actions", x, *_head(x, bound), C.byref(k), actions.data_ptr(), log_prob.data_ptr(),
+          ws.data_ptr() if nbytes else None, nbytes)
+    return ActionSample(actions, log_prob)
 
 
-@_on_device
-def _score_backward(x, rules, actions, lp, ent, lse, g_lp, g_ent):
-    ref, _, keep = _bound(rules, x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    g_lp = None if g_lp is None else g_lp.contiguous()
-    g_ent = None if g_ent is None else g_ent.contiguous()
-    L.check(L.load().gymhip_action_log_prob_backward(x.data_ptr(), _TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), ref, actions.data_ptr(),
-                                                     _INTS[actions.dtype], lp.data_ptr(), ent.data_ptr(), lse.data_ptr(),
-                                                     None if g_lp is None else g_lp.data_ptr(), None if g_ent is None else g_ent.data_ptr(), out.data_ptr(),
-                                                     out.stride(0), _raw_stream(x.device)), "gymhip_action_log_prob_backward")
-    return out
+def _score(x, bound, actions):
+    n, width = x.shape
+    device = x.device
+    nbytes = (_lib or _load()).gymhip_action_log_prob_workspace_bytes(n, width)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    lp, ent = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
+    log_sum = torch.empty(n, 2, dtype=torch.float64, device=device)
+    _call("gymhip_action_log_prob", x, *_head(x, bound), actions.data_ptr(), _INTS[actions.dtype], lp.data_ptr(), ent.data_ptr(), log_sum.data_ptr(),
+          ws.data_ptr() if nbytes else None, nbytes)
+    return lp, ent, log_sum
 
 
 class _Score(torch.autograd.Function):
@@ -328,64 +321,66 @@ class _Score(torch.autograd.Function):
     def forward(ctx, logits, actions, rules):
         ctx.set_materialize_grads(False)
         x = _rowwise(logits)
-        lp, ent, lse = _score(x, rules, actions)
-        _save(ctx, rules, x, actions, lp, ent, lse)
+        bound = _bind(rules, x)
+        lp, ent, log_sum = _score(x, bound, actions)
+        _save(ctx, rules, bound, x, actions, lp, ent, log_sum)
         return lp, ent
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent):
-        x, actions, lp, ent, lse = ctx.saved_tensors[:5]
-        return _score_backward(x, ctx.rules, actions, lp, ent, lse, g_lp, g_ent), None, None
+        _once()
+        x, actions, lp, ent, log_sum = ctx.saved_tensors[:5]
+        x = _rowwise(x)
+        out = _empty_like(x)
+        g_lp, g_ent = (g if g is None or g.is_contiguous() else g.contiguous() for g in (g_lp, g_ent))
+        _call("gymhip_action_log_prob_backward", x, *_head(x, ctx.bound), actions.data_ptr(), _INTS[actions.dtype], lp.data_ptr(), ent.data_ptr(),
+              log_sum.data_ptr(), None if g_lp is None else g_lp.data_ptr(), None if g_ent is None else g_ent.data_ptr(),
+              out.data_ptr(), out.stride(0))
+        return out, None, None
 
 
 def action_log_prob(logits: torch.Tensor, actions: torch.Tensor, rules: LogitRules | None = None):
     """(log softmax(z)[action], entropy of softmax(z)), float32 [rows] each, for logits [rows, width] and actions int32 / int64 [rows].
     Differentiable in the logits.  An action that is not allowed, or outside [0, width), has -inf and hands no gradient back through its
     log-probability; a row with nothing allowed has -inf, entropy 0 and no gradient."""
-    _matrix(logits, "logits")
-    _checked(rules)
-    actions = _side(actions, "actions", logits.device, (torch.int32, torch.int64), ((logits.shape[0],),))
+    x = _ready(logits, rules)
+    actions = _side(actions, "actions", x.device, (torch.int32, torch.int64), ((x.shape[0],),))
     if logits.requires_grad and torch.is_grad_enabled():
         return _Score.apply(logits, actions, rules)
-    return _score(_rowwise(logits), rules, actions)[:2]
+    return _score(x, _bind(rules, x), actions)[:2]
 
 
-@_on_device
-def _drop(x, p, seed, step, rows, out):
-    k, keep = _keys(x.shape[0], x.device, seed, step, rows)
-    L.check(L.load().gymhip_dropout(x.data_ptr(), _TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), p, C.byref(k), out.data_ptr(), out.stride(0),
-                                    _raw_stream(x.device)), "gymhip_dropout")
+def _drop(x, p, keys):
+    n, width = x.shape
+    out = _empty_like(x)
+    _call("gymhip_dropout", x, x.data_ptr(), _TYPES[x.dtype], n, width, x.stride(0), p, C.byref(keys), out.data_ptr(), out.stride(0))
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, p, seed, step, rows):
-        ctx.args = (p, seed)
-        ctx.numbers = (None if isinstance(step, torch.Tensor) else step, None if isinstance(rows, torch.Tensor) else rows)
-        ctx.save_for_backward(*(t for t in (step, rows) if isinstance(t, torch.Tensor)))
-        x = _rowwise(x)
-        return _drop(x, p, seed, step, rows, torch.empty(x.shape, dtype=x.dtype, device=x.device))
+    def forward(ctx, x, p, keys, *tensors):
+        ctx.p, ctx.keys, ctx.tensors = p, keys, tensors   # keys point into the tensors
+        if tensors:   # a change in place before the backward pass raises
+            ctx.save_for_backward(*tensors)
+        return _drop(_rowwise(x), p, keys)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        saved = list(ctx.saved_tensors)
-        step, rows = (saved.pop(0) if v is None else v for v in ctx.numbers)
-        g = _rowwise(grad)
-        return _drop(g, *ctx.args, step, rows, torch.empty(g.shape, dtype=g.dtype, device=g.device)), None, None, None, None
+        _once()
+        saved = ctx.saved_tensors
+        return (_drop(_rowwise(grad), ctx.p, ctx.keys),) + (None,) * (2 + len(saved))
 
 
 def dropout(x: torch.Tensor, p: float, *, seed: int, step=0, rows=0) -> torch.Tensor:
     """x [rows, width] with each element 0 with probability p (p to 16 bits: t = round(65536 p)) and multiplied by 65536 / (65536 - t)
     otherwise.  Which ones follows from (seed, row key, step, column) alone (`rows` and `step` as in sample_actions); give every layer a
     seed of its own.  Differentiable in x; the backward pass draws the mask again, so a device `step` must not be advanced before it."""
-    _matrix(x, "x")
+    matrix = _ready(x, None, "x")
     p = float(p)
     if not 0.0 <= p < 1.0 or round(65536 * p) > 65535:
         raise ValueError(f"p must lie in [0, 1) and round to less than 65536 / 65536, got {p}")
+    keys, tensors = _keys(matrix.shape[0], matrix.device, seed, step, rows)
     if x.requires_grad and torch.is_grad_enabled():
-        return _Dropout.apply(x, p, seed, step, rows)
-    x = _rowwise(x)
-    return _drop(x, p, seed, step, rows, torch.empty(x.shape, dtype=x.dtype, device=x.device))
+        return _Dropout.apply(x, p, keys, *tensors)
+    return _drop(matrix, p, keys)

@@ -554,3 +554,33 @@ def test_captured_and_replayed(width, n):
             assert torch.equal(a, b)
         seen.append(out.actions.clone())
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_saved_tensors_may_move_before_the_backward_pass():
+    """Hooks that keep saved tensors elsewhere (here: on the host) hand back other memory than the forward pass read."""
+    from gym_amd.policy import action_log_prob, process_logits
+    x, g = logits_of(6, 700, torch.float32, 5)
+    rules = rules_of("all", 6, 700, g)
+    a = torch.arange(6).cuda()
+
+    def gradients(moved):
+        leaf = x.detach().clone().requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if moved else torch.enable_grad():
+            y = leaf * 1.0
+            z = process_logits(y, rules)
+            lp, ent = action_log_prob(y, a, rules)
+        del y
+        junk = [torch.full((6, 700), math.nan, device="cuda") for _ in range(8)]   # whatever was freed is used again
+        out = torch.autograd.grad(torch.where(torch.isinf(z), 0.0, z).sum() + lp.nan_to_num(neginf=0).sum() + ent.sum(), leaf)[0]
+        del junk
+        return out
+
+    assert torch.equal(gradients(True), gradients(False))
+
+
+def test_second_derivatives_are_refused():
+    from gym_amd.policy import action_log_prob
+    x, _ = logits_of(2, 5, torch.float32, 5)
+    leaf = x.detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(action_log_prob(leaf, torch.zeros(2, dtype=torch.int32, device="cuda"))[1].sum(), leaf, create_graph=True)
