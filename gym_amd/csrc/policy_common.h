@@ -168,10 +168,27 @@ __device__ inline uint4 row_words(const Keys& k, int64_t b, uint32_t block) {
 // The draw's u: 52 random bits and a half, so that every value is exact in a double and neither 0 nor 1 occurs.
 __device__ inline double row_uniform(const Keys& k, int64_t b) {
     const uint4 w = row_words(k, b, 0xFFFFFFFFu);   // a block that no column has
-    return ((double)(((uint64_t)w.x << 20) | (w.y >> 12)) + 0.5) * 0x1p-52;
+    const double one_to_two = __hiloint2double((int)(0x3FF00000u | w.x >> 12), (int)(w.x << 20 | w.y >> 12));
+    return one_to_two - 1.0 + 0x1p-53;
 }
 
 // ---- rules ---------------------------------------------------------------------------------------------------------------------------
+// What a temperature makes of exponentials: exp(y / temp) is 2^(y k2).  From `least` on down that is below 2^-1000, up to `most` at most 2^900.
+struct Heat {
+    double temp, k2, least, most;
+    bool greedy;
+    static __host__ __device__ Heat of(float t) {
+        Heat h;
+        h.greedy = !(t > 0.f);
+        h.temp = h.greedy ? 1.0 : t < 3e38f ? (double)t : 3e38;
+        h.k2 = 1.4426950408889634074 / h.temp;
+        const double unit = h.temp * 0.69314718055994530942, most = 900.0 * unit;
+        h.least = -1000.0 * unit;
+        h.most = most < 3e38 ? most : 3e38;   // an infinite logit is above it
+        return h;
+    }
+};
+
 struct Rules {
     const uint32_t* mask;
     int64_t mask_stride, mask_lines;
@@ -184,26 +201,30 @@ struct Rules {
     uint32_t hist_cols;
     int hist64, len64;
     const float *rep_rows, *pres_rows, *freq_rows, *temp_rows;
-    float rep, pres, freq, temp;
+    float rep, pres, freq;
+    Heat heat;   // of the one temperature where temp_rows is null, made on the host
     // y is the logit itself, or -inf where the mask does not allow it
     __host__ __device__ bool plain() const { return !bias && !hist; }
 };
 
 // One row's share of them.
-struct Row {
+struct Row : Heat {
     const uint32_t* mask;   // its line, or null where everything is allowed
     const float* bias;
-    double rep, inv_rep, pres, freq, temp;
-    bool greedy, nothing;   // nothing: its line lies behind the mask's last one
+    double rep, inv_rep, pres, freq;
+    bool masked, biased;    // there is a mask, a bias at all: the same for all rows
+    bool nothing;           // its line lies behind the mask's last one
 };
 
 // RULES: there is a bias or a history.
 template <bool RULES>
 __device__ inline Row row_of(const Rules& r, int64_t b) {
     Row w;
-    const float t = r.temp_rows ? r.temp_rows[b] : r.temp;
-    w.greedy = !(t > 0.f);
-    w.temp = w.greedy ? 1.0 : t < 3e38f ? (double)t : 3e38;
+    // (all of it in the branch: a temperature of its own costs a division)
+    if (r.temp_rows) (Heat&)w = Heat::of(r.temp_rows[b]);
+    else (Heat&)w = r.heat;
+    w.masked = r.mask != nullptr;
+    w.biased = RULES && r.bias;
     w.mask = nullptr;
     w.bias = nullptr;
     w.nothing = false;
@@ -236,11 +257,11 @@ __device__ inline double divided(double x, double d, double inv) {
 
 // The mask's bits of C (at most 8) columns from v0 on, v0 a multiple of C; of none behind the row's end.
 __device__ inline uint32_t allowed_bits(const Row& w, int64_t v0, int64_t width) {
+    if (!w.masked) return 0xFFu;
     if (w.nothing) return 0u;
     return w.mask && v0 < width ? w.mask[v0 >> 5] >> (v0 & 31) : 0xFFu;
 }
 
-__device__ inline bool has_mask(const Row& w) { return w.mask || w.nothing; }
 __device__ inline bool allowed(const Row& w, int64_t v) { return !w.nothing && (!w.mask || (w.mask[v >> 5] >> (v & 31) & 1u)); }
 
 // x under the penalties of a count > 0.
@@ -252,7 +273,7 @@ __device__ inline double penalised(const Row& w, double x, uint32_t count) {
 __device__ inline double ruled(const Row& w, float xf, uint32_t count, bool ok, int64_t v) {
     double y = xf;
     if (count) y = penalised(w, y, count);
-    if (w.bias) y += (double)w.bias[v];
+    if (w.biased) y += (double)w.bias[v];
     return ok ? y : -INFINITY;
 }
 
@@ -341,7 +362,7 @@ __device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, uint32_t b
             }
         }
     }
-    if (w.bias) {
+    if (w.biased) {
         float f[C];
         bias_cols<C>(w, v0, width, f);
 #pragma unroll
@@ -503,7 +524,7 @@ int check_actions(const void* actions, int dtype, int64_t rows);
 int check_workspace(const void* workspace, size_t bytes, size_t needed);
 int launched();
 
-// Workgroups for n units of work: as many as there are, up to what keeps every CU busy several times over; kernels stride over the rest.
+// Workgroups for n units of work: as many as there are, up to `most`; kernels stride over the rest.
 inline unsigned grid_for(int64_t n, int64_t most = 1 << 16) { return (unsigned)(n < most ? n : most); }
 
 // f(E{}) for the element type of `type`.

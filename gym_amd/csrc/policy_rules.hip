@@ -71,20 +71,15 @@ __device__ inline void each_vector(const Rules& r, const Tiling& t, const typena
         } else {
             if (b >= rows) continue;
             Raw<E, C> raw[kTile];
-            uint32_t bits[kTile];
 #pragma unroll
             for (int k = 0; k < kTile; k++)
                 if (k < t.nv && v0 + k * step < width) raw[k].load(from, v0 + k * step, width);
             const auto state = begin(b);
-            if (has_mask(state)) {
-#pragma unroll
-                for (int k = 0; k < kTile; k++) bits[k] = allowed_bits(state, v0 + k * step, width);
-            }
 #pragma unroll
             for (int k = 0; k < kTile; k++) {
                 const int64_t at = v0 + k * step;
                 if (k >= t.nv || at >= width) continue;
-                f(state, raw[k], b, at, bits[k], 0, 0u);
+                f(state, raw[k], b, at, 0u, 0, 0u);
                 raw[k].store(to, at, width);
             }
         }
@@ -96,17 +91,34 @@ __device__ inline void each_vector(const Rules& r, const Tiling& t, const typena
     __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];                  \
     const Counts counts { RULES && r.hist ? words : nullptr, (E::kVec << t.lanes_log2) * t.nv, kBlock * E::kVec * t.nv, t.half, t.lanes_log2 >= 3 }
 
-// x / d of floats as IEEE rounds it.  inv = 1 / d, or 0 where d is not between 2^-20 and 2^20: then, and where the quotient is not between 2^-60 and
-// 2^100, the remainder may not be exact (see the double's `divided`) and the division itself is made.
-__device__ inline float dividedf(float x, float d, float inv) {
-    const float q = x * inv, a = fabsf(q);
-    if (a > 0x1p-60f && a < 0x1p100f) return __builtin_fmaf(__builtin_fmaf(-q, d, x), inv, q);
-    return (x == 0.f || fabsf(x) == INFINITY) ? x : x / d;
+// z = x / d of floats as IEEE rounds it (z may be x).  inv = 1 / d, or 0 where d is not between 2^-20 and 2^20: then, and where the quotient is not
+// between 2^-60 and 2^100, the remainder may not be exact (see `divided`) and the division itself is made.  Straight-line code but for lanes that
+// hold such a quotient: a zero, an infinity, or what hardly occurs.
+template <int C>
+__device__ inline void divide_cols(const float* x, float d, float inv, float* z) {
+    bool odd = false;
+    float c[C];
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        const float q = x[j] * inv, a = fabsf(q);
+        c[j] = __builtin_fmaf(__builtin_fmaf(-q, d, x[j]), inv, q);
+        odd = odd || !(a > 0x1p-60f && a < 0x1p100f);
+    }
+    if (odd) {
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            const float a = fabsf(x[j] * inv);
+            if (!(a > 0x1p-60f && a < 0x1p100f)) c[j] = x[j] == 0.f || fabsf(x[j]) == INFINITY ? x[j] : x[j] / d;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < C; j++) z[j] = c[j];
 }
 
 struct ProcessRow : Row {
     double inv_temp;
     float tempf, inv_tempf;
+    bool undivided;   // every row's temperature is 1 (or 0)
 };
 template <bool RULES>
 __device__ inline ProcessRow process_row(const Rules& r, int64_t b) {
@@ -114,6 +126,7 @@ __device__ inline ProcessRow process_row(const Rules& r, int64_t b) {
     (Row&)p = row_of<RULES>(r, b);
     p.inv_temp = 1.0 / p.temp;
     p.tempf = (float)p.temp;
+    p.undivided = !r.temp_rows && r.heat.temp == 1.0;
     p.inv_tempf = p.tempf >= 0x1p-20f && p.tempf <= 0x1p20f ? 1.f / p.tempf : 0.f;
     return p;
 }
@@ -128,14 +141,15 @@ __global__ void __launch_bounds__(kBlock) process_kernel(const typename E::T* x,
                           [&](const ProcessRow& p, Raw<E, C>& raw, int64_t, int64_t at, uint32_t bits, int place, uint32_t apart) {
         float z[C];
         const Raw<E, C> whole = raw;
-        if (RULES && p.bias) {
+        if (RULES && p.biased) {
             float f[C];
             bias_cols<C>(p, at, width, f);
 #pragma unroll
             for (int j = 0; j < C; j++) z[j] = (float)divided((double)raw.get(j) + (double)f[j], p.temp, p.inv_temp);
         } else {
 #pragma unroll
-            for (int j = 0; j < C; j++) z[j] = dividedf(raw.get(j), p.tempf, p.inv_tempf);
+            for (int j = 0; j < C; j++) z[j] = raw.get(j);
+            if (!p.undivided) divide_cols<C>(z, p.tempf, p.inv_tempf, z);
         }
         raw.set(z);
         if (RULES) {
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(kBlock) process_kernel(const typename E::T* x,
                 raw.put(j, (float)divided(ruled(p, whole.pick(j), counts.at(place + j), true, at + j), p.temp, p.inv_temp));
             }
         }
-        if (has_mask(p)) raw.keep(bits);
+        if (p.masked) raw.keep(RULES ? bits : allowed_bits(p, at, width));
     });
 }
 
@@ -160,7 +174,8 @@ __global__ void __launch_bounds__(kBlock) process_backward_kernel(const typename
         float u[C];
         const Raw<E, C> whole = raw;
 #pragma unroll
-        for (int j = 0; j < C; j++) u[j] = dividedf(raw.get(j), p.tempf, p.inv_tempf);
+        for (int j = 0; j < C; j++) u[j] = raw.get(j);
+        if (!p.undivided) divide_cols<C>(u, p.tempf, p.inv_tempf, u);
         raw.set(u);
         if (RULES) {
             while (apart) {
@@ -170,7 +185,7 @@ __global__ void __launch_bounds__(kBlock) process_backward_kernel(const typename
                 raw.put(j, (float)((double)whole.pick(j) * (xf > 0.f ? p.inv_rep : p.rep) * p.inv_temp));
             }
         }
-        if (has_mask(p)) raw.clear(bits);
+        if (p.masked) raw.clear(RULES ? bits : allowed_bits(p, at, width));
     });
 }
 
@@ -206,7 +221,7 @@ __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E
         s.empty = ls == -INFINITY;
         s.ls2 = (float)(ls * kLog2e);
         s.inv_temp = (float)(1.0 / s.temp);
-        s.k = (float)(kLog2e / s.temp);
+        s.k = (float)s.k2;
         s.gl = !g_lp || log_prob[b] == -INFINITY ? 0.f : g_lp[b];
         s.ge = g_ent ? g_ent[b] : 0.f;
         s.ent = entropy[b];
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E
         const int64_t hot = s.act - at;
         float g[C];
         const Raw<E, C> whole = raw;
-        if (RULES && s.bias) {
+        if (RULES && s.biased) {
             float f[C];
             bias_cols<C>(s, at, width, f);
 #pragma unroll
@@ -242,7 +257,7 @@ __global__ void __launch_bounds__(kBlock) score_backward_kernel(const typename E
             }
         }
         if (s.empty) raw.clear(0u);
-        else if (has_mask(s)) raw.clear(bits);
+        else if (s.masked) raw.clear(RULES ? bits : allowed_bits(s, at, width));
     });
 }
 
@@ -274,7 +289,8 @@ int check_output(const char* what, const void* out, int type, int64_t rows, int6
 
 int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules* out) {
     *out = Rules{};
-    out->rep = out->temp = 1.f;
+    out->rep = 1.f;
+    out->heat = Heat::of(1.f);
     if (!r) return GYMHIP_OK;
     if (r->struct_size != (int32_t)sizeof(gymhip_logit_rules)) return fail(GYMHIP_EINVAL, "bad gymhip_logit_rules.struct_size");
     if (r->mask) {
@@ -304,7 +320,8 @@ int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules*
         out->hist64 = r->history_dtype == GYMHIP_ACT_I64; out->len64 = r->history_len_dtype == GYMHIP_ACT_I64;
     }
     out->rep_rows = r->repetition_rows; out->pres_rows = r->presence_rows; out->freq_rows = r->frequency_rows; out->temp_rows = r->temperature_rows;
-    out->rep = r->repetition; out->pres = r->presence; out->freq = r->frequency; out->temp = r->temperature;
+    out->rep = r->repetition; out->pres = r->presence; out->freq = r->frequency; 
+    if (!r->temperature_rows) out->heat = Heat::of(r->temperature);
     return GYMHIP_OK;
 }
 

@@ -10,16 +10,8 @@ namespace gymhip {
 namespace policy {
 namespace {
 
-// What a row's temperature makes of the exponentials: a weight is 2^(d k2), d = y - base.  Below `least` it counts as none (2^-1000); up to
-// `most` it is at most 2^900.
-struct Scale {
-    double k2, least, most;
-};
-__device__ inline Scale scale_of(const Row& w) {
-    const double unit = w.temp * kLn2;
-    return Scale{kLog2e / w.temp, -1000.0 * unit, fmin(900.0 * unit, 3e38)};   // an infinite logit never fits
-}
-__device__ inline double weight(double d, const Scale& c) { return exp2_double(__builtin_fmax(d, c.least), c.k2); }
+// A weight: 2^(d k2), d = y - base.
+__device__ inline double weight(double d, const Heat& c) { return exp2_double(__builtin_fmax(d, c.least), c.k2); }
 
 // Where a lane stands in its row: `at` its first column, `step` the columns from one of its vectors to the next, `place` its first column's place in
 // the counts.
@@ -36,14 +28,14 @@ template <typename E, bool RULES, int C, typename F>
 __device__ inline void with_y(const Row& w, const Place& p, int k, Vector<E, C> v, F f) {
     if constexpr (RULES) {
         const bool counted = p.counts.any<C>(p.place + k * p.step);
-        if (counted || w.bias) {
+        if (counted || w.biased) {
             double y[C];
             ruled_cols(w, v.raw, v.bits, p.at + k * p.step, p.width, p.counts, p.place + k * p.step, counted, y);
             f(y);
             return;
         }
     }
-    if (has_mask(w)) v.raw.keep(v.bits);
+    if (w.masked) v.raw.keep(v.bits);
     float y[C];
 #pragma unroll
     for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
@@ -52,7 +44,7 @@ __device__ inline void with_y(const Row& w, const Place& p, int k, Vector<E, C> 
 
 // A vector's weights e against `base`, and their sum.
 template <int C, typename Y>
-__device__ inline double weigh(const Y* y, double base, const Scale& c, double* e) {
+__device__ inline double weigh(const Y* y, double base, const Heat& c, double* e) {
     double s = 0;
 #pragma unroll
     for (int j = 0; j < C; j++) s += e[j] = weight((double)y[j] - base, c);
@@ -62,7 +54,7 @@ __device__ inline double weigh(const Y* y, double base, const Scale& c, double* 
 // is to do where no y is above `most` nor a NaN and the row's sum is not below 2^-900.  *beyond: the wave's lanes that have such a y (as a lane mask: one
 // vector instruction a column).
 template <int C, typename Y>
-__device__ inline double weigh_0(const Y* y, const Scale& c, double* e, uint64_t* beyond) {
+__device__ inline double weigh_0(const Y* y, const Heat& c, double* e, uint64_t* beyond) {
     double s = 0;
 #pragma unroll
     for (int j = 0; j < C; j++) {
@@ -74,7 +66,7 @@ __device__ inline double weigh_0(const Y* y, const Scale& c, double* e, uint64_t
 // The sum of vector k's weights against 0, in no order of columns: the few columns with a count are left out of the straight pass, which then is no
 // dearer than one without a history, and each is gone through by itself afterwards by the lane that owns it.
 template <typename E, bool RULES>
-__device__ inline double weigh_apart(const Row& w, const Place& p, int k, Vector<E, E::kVec> v, const Scale& c, uint64_t* beyond) {
+__device__ inline double weigh_apart(const Row& w, const Place& p, int k, Vector<E, E::kVec> v, const Heat& c, uint64_t* beyond) {
     constexpr int C = E::kVec;
     double e[C];
     if constexpr (!RULES) {
@@ -86,9 +78,9 @@ __device__ inline double weigh_apart(const Row& w, const Place& p, int k, Vector
         const int place = p.place + k * p.step;
         uint32_t apart = p.counts.words ? p.counts.which<C>(place) & v.bits : 0u;
         const Raw<E, C> whole = v.raw;
-        if (has_mask(w) || __any(apart)) v.raw.keep(v.bits & ~apart);
+        if (w.masked || __any(apart)) v.raw.keep(v.bits & ~apart);
         double s;
-        if (w.bias) {
+        if (w.biased) {
             float f[C];
             double y[C];
             bias_cols<C>(w, at, p.width, f);
@@ -121,7 +113,7 @@ struct Mass {
 // The greatest y of a group's columns (nv vectors a lane), whatever it is (-inf: there is none at all), the sum against it, and the first column that
 // holds it: for greedy rows, and the rare ones out of weigh_0's range.
 template <typename E, bool RULES, int G, int C>
-__device__ inline Mass sum_against_max(const typename E::T* x, const Row& w, const Place& p, int nv, const Scale& c, double* lds, long long* first) {
+__device__ inline Mass sum_against_max(const typename E::T* x, const Row& w, const Place& p, int nv, const Heat& c, double* lds, long long* first) {
     double m = -INFINITY, sum = 0;
     int best = 0;
     bool bad = false;
@@ -182,16 +174,18 @@ __device__ inline int walk(const double* e, double s, double before, double leve
     }
     // every lane walks its own vector; the chosen lane's answer counts
     double acc = before + (upto - s);
-    int at = -1, last = 0;
+    int at = C;
 #pragma unroll
     for (int j = 0; j < C; j++) {
         acc += e[j];
-        if (e[j] > tiny) {
-            last = j;
-            if (at < 0 && acc > level) at = j;
-        }
+        at = at == C && acc > level ? j : at;
     }
-    if (at < 0) at = last;
+    if (__any(at == C)) {
+        int last = 0;
+#pragma unroll
+        for (int j = 0; j < C; j++) last = e[j] > tiny ? j : last;
+        at = at == C ? last : at;
+    }
     if (W > 1) at = __shfl(at, first);
     return (first & (W - 1)) * C + at;
 }
@@ -200,7 +194,7 @@ __device__ inline float log_prob_of(double y, double m, double k2, double sum) {
 
 // A row's answer, by one lane: `at` its chosen column unless there is none.
 template <typename E>
-__device__ inline void answer(const Row& w, const typename E::T* x, const Mass& mass, int64_t at, uint32_t count, const Scale& c, int64_t b,
+__device__ inline void answer(const Row& w, const typename E::T* x, const Mass& mass, int64_t at, uint32_t count, const Heat& c, int64_t b,
                               int32_t* actions, float* log_prob) {
     const bool none = mass.bad || mass.base == -INFINITY;
     actions[b] = none ? -1 : (int32_t)at;
@@ -226,7 +220,7 @@ __global__ void __launch_bounds__(kBlock) sample_vectors_kernel(const typename E
         Vector<E, C> v;
         v.load(w, x, p.at, width);
         if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
-        const Scale c = scale_of(w);
+        const Heat c = w;
         double s = 0, e[C];
         uint64_t beyond = 0;
         with_y<E, RULES, C>(w, p, 0, v, [&](const auto* y) { s = weigh_0<C>(y, c, e, &beyond); });
@@ -261,7 +255,7 @@ __device__ inline void each_vector(const Row& w, const typename E::T* x, const P
 
 // sums[k * waves + wave]: the sum of each wave's k-th vectors against `base`.  v0: this lane's first vector.
 template <typename E, bool RULES, int G>
-__device__ inline void strip_sums(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Scale& c, double base,
+__device__ inline void strip_sums(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Heat& c, double base,
                                   double* sums) {
     constexpr int C = E::kVec, M = G / kWave;
     const int wave = G > kWave ? (int)threadIdx.x / kWave : 0;
@@ -277,7 +271,7 @@ __device__ inline void strip_sums(const typename E::T* x, const Vector<E, E::kVe
 
 // The sum of a strip.
 template <typename E, bool RULES, int G>
-__device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Scale& c, double* lds,
+__device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Heat& c, double* lds,
                                  long long* first) {
     constexpr int C = E::kVec;
     if (!w.greedy) {   // one row's: all lanes alike
@@ -293,7 +287,7 @@ __device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec
 // The column of a strip (0 = its first) that the running sum passes `level` in; sums as strip_sums left them for the same base, which is finite, and
 // `sum` the strip's.
 template <typename E, bool RULES, int G>
-__device__ inline int locate(const typename E::T* x, const Row& w, const Place& p, int nv, const Scale& c, double base, double sum, double level,
+__device__ inline int locate(const typename E::T* x, const Row& w, const Place& p, int nv, const Heat& c, double base, double sum, double level,
                              const double* sums, int* lds_at) {
     constexpr int C = E::kVec, M = G / kWave;
     const int wave = G > kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave) : 0;
@@ -356,7 +350,7 @@ __global__ void __launch_bounds__(kBlock) sample_strips_kernel(const typename E:
         Vector<E, C> v;
         v.load(w, x, p.at, width);
         if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
-        const Scale c = scale_of(w);
+        const Heat c = w;
         long long first = 0;
         const Mass mass = sum_strip<E, RULES, G>(x, v, w, p, nv, c, lds, &first);
         int64_t at = first;
@@ -393,7 +387,7 @@ __global__ void __launch_bounds__(kBlock) sample_parts_kernel(const typename E::
         v.load(w, x, p.at, width);
         if (hist) count_ids(r, b, 1, rows, width, lo, counts);
         long long first = 0;
-        const Mass mass = sum_strip<E, RULES, kBlock>(x, v, w, p, nv, scale_of(w), lds, &first);
+        const Mass mass = sum_strip<E, RULES, kBlock>(x, v, w, p, nv, w, lds, &first);
         if (threadIdx.x == 0) parts[b * cuts + blockIdx.x] = Part{mass.base, mass.bad ? (double)NAN : mass.base == -INFINITY ? 0.0 : mass.sum, first};
     }
 }
@@ -413,7 +407,7 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
     for (int64_t b = blockIdx.x; b < rows; b += gridDim.x) {
         const Part* parts_b = parts + b * cuts;
         const Row w = row_of<RULES>(r, b);
-        const Scale scale = scale_of(w);
+        const Heat scale = w;
         const typename E::T* x = x0 + b * stride;
         const double u = row_uniform(keys, b);
         double m = -INFINITY;
@@ -511,7 +505,7 @@ struct Launch {
     template <int G, int C>
     void vectors() const {
         constexpr int per = kBlock / G;
-        hipLaunchKernelGGL((sample_vectors_kernel<E, RULES, G, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r, k,
+        hipLaunchKernelGGL((sample_vectors_kernel<E, RULES, G, C>), dim3(grid_for((rows + per - 1) / per, 4096)), dim3(kBlock), 0, s, x, rows, width, stride, r, k,
                            actions, log_prob);
     }
     template <int G>

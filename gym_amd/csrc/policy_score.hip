@@ -87,14 +87,14 @@ __device__ inline void add_columns(Run& run, const Row& w, const typename E::T* 
                 // the few columns with a count are left out of the straight pass, and each is added by itself by the lane that owns it
                 uint32_t apart = counts.words ? counts.which<C>(place + k * step) & v.bits : 0u;
                 const Raw<E, C> whole = v.raw;
-                if (has_mask(w) || __any(apart)) v.raw.keep(v.bits & ~apart);
-                if (w.bias) {
+                if (w.masked || __any(apart)) v.raw.keep(v.bits & ~apart);
+                if (w.biased) {
                     float f[C];
                     double y[C];
                     bias_cols<C>(w, at, width, f);
 #pragma unroll
                     for (int j = 0; j < C; j++) y[j] = (double)v.raw.get(j) + (double)f[j];
-                    if (has_mask(w)) {   // whatever the bias is there
+                    if (w.masked) {   // whatever the bias is there
 #pragma unroll
                         for (int j = 0; j < C; j++) y[j] = v.bits >> j & 1 ? y[j] : -INFINITY;
                     }
@@ -118,14 +118,14 @@ __device__ inline void add_columns(Run& run, const Row& w, const typename E::T* 
         uint32_t bits[NV];
 #pragma unroll
         for (int k = 0; k < NV; k++) raw[k].load(x, first + k * step, NV == 1 || first + k * step < width ? width : 0);
-        if (has_mask(w)) {
+        if (w.masked) {
 #pragma unroll
             for (int k = 0; k < NV; k++) bits[k] = allowed_bits(w, first + k * step, width);
         }
         float y[NV * C];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            if (has_mask(w)) raw[k].keep(bits[k]);
+            if (w.masked) raw[k].keep(bits[k]);
 #pragma unroll
             for (int j = 0; j < C; j++) y[k * C + j] = raw[k].get(j);
         }
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kBlock) score_rows_kernel(const typename E::T*
         const int64_t b = own < rows ? own : rows - 1;   // lanes without a row follow the last one: every exchange has all its lanes
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const double k2 = kLog2e / w.temp;
+        const double k2 = w.k2;
         Run run{-INFINITY, 0, 0, 0};
         add_columns<E, RULES, NV, C>(run, w, x, lane * C, G * C, nv, width, counts, group * cap + lane * C, k2, [&] {
             if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kBlock) score_wide_kernel(const typename E::T*
         const int64_t c0 = part * each, c1 = c0 + each < cuts ? c0 + each : cuts;
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const double k2 = kLog2e / w.temp;
+        const double k2 = w.k2;
         const int64_t a = action_of(actions, act64, b);
         Run run{-INFINITY, 0, 0, 0};
         if (threadIdx.x == 0) the_ya = -INFINITY;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
         const Row w = row_of<false>(r, b);
         Run run{-INFINITY, 0, 0, 0};
         if (lane < splits) run = parts[b * splits + lane].run;
-        join<kWave>(run, kLog2e / w.temp, nullptr);
+        join<kWave>(run, w.k2, nullptr);
         if (lane == 0 && own < rows) {
             const int64_t a = action_of(actions, act64, b);
             finish(run, w, a >= 0 && a < width ? parts[b * splits + a / cap / each].ya : -INFINITY, b, log_prob, entropy, log_sum);
