@@ -8,6 +8,8 @@ Same names, argument meaning and error behaviour as the C++ templates it stands 
     gym::VecNormalize<false, training, normReward, normObs>   wrappers/vec_env/vec_normalize.h -> VecNormalize
     gym::VecFrameStack / VecNormAndPermute                     vec_frame_stack.cpp, vec_atari.cpp -> gym_amd.atari
 
+VecLogitActions (step takes a policy's logits) and VecObservationDropout have no counterpart there: the reference leaves both to its trainer.
+
 The per-env wrappers are not objects here: TimeLimit / ClipReward / Monitor (and VecNormalize) are flags of ONE fused
 kernel.  Returned tensors are views of device buffers that the next step overwrites (the reference allocates fresh
 tensors every step, sync_env.h:107-112) — clone what you keep.
@@ -349,6 +351,118 @@ class VecEnvWrapper(VecEnv):
 
     def seed(self, _seed):
         return self.venv.seed(_seed)
+
+
+def _env_offset(venv):
+    """The global index of the first env under any wrappers: the random-number key of row 0."""
+    while not hasattr(venv, "env_offset") and hasattr(venv, "venv"):
+        venv = venv.venv
+    return int(getattr(venv, "env_offset", 0))
+
+
+class _Counter:
+    """The step number of the random draws: on the host, or (device=True) an int64 scalar on the GPU that the stream itself advances, so that a
+    recorded graph draws anew at every replay (one more launch per step)."""
+
+    def __init__(self, device: bool):
+        self._on_device, self.value = bool(device), 0
+
+    def restart(self):
+        if isinstance(self.value, torch.Tensor):
+            self.value.zero_()   # in place: a recorded graph goes on with the same scalar
+        else:
+            self.value = 0
+
+    def on(self, device):
+        """The number to draw with, for tensors on `device`."""
+        if device.type == "cuda" and not isinstance(self.value, torch.Tensor) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a recorded graph would draw the same at every replay: make the wrapper with device_step=True and take a step before recording"
+                               if not self._on_device else "take a step before recording")
+        if self._on_device and not isinstance(self.value, torch.Tensor):
+            self.value = torch.full((), self.value, dtype=torch.int64, device=device)
+        return self.value
+
+    def advance(self):
+        if isinstance(self.value, torch.Tensor):
+            self.value.add_(1)
+        else:
+            self.value += 1
+
+
+class VecLogitActions(VecEnvWrapper):
+    """step(logits [N, n]) over a VecEnv with a Discrete(n) action space: one action per env from softmax(logits) under `rules`
+    (gym_amd.policy.LogitRules; may be assigned between steps) is drawn on the GPU and handed to the engine as it is (int32, no copy).
+
+    The draw of env i at step t follows from (seed, i's GLOBAL index, t) alone: neither the GPU count nor the order of the calls matters.
+    seed(s) gives the envs their seeds and the draws a new one, and restarts t.  `sample` holds the last step's actions and log-probabilities
+    (new tensors each step); action_log_prob scores them again, with gradients.  An env whose rules leave nothing to choose gets action -1.
+    device_step=True keeps t on the GPU, for steps recorded into a graph."""
+
+    def __init__(self, venv: VecEnv, rules=None, seed: int = 0, device_step: bool = False):
+        super().__init__(venv)
+        if not isinstance(venv.actionSpace(), spaces.Discrete):
+            raise TypeError(f"VecLogitActions needs a Discrete action space, got {venv.actionSpace()!r}")
+        self.rules, self.sample = rules, None
+        self._seed, self._step, self._offset = int(seed), _Counter(device_step), _env_offset(venv)
+
+    def seed(self, _seed):
+        self._seed = int(_seed)
+        self._step.restart()
+        return self.venv.seed(_seed)
+
+    def stepAsync(self, logits):
+        from . import policy
+        shape = (self.numEnvs, self.actionSpace().n)
+        if tuple(logits.shape) != shape:
+            raise ValueError(f"logits have shape {tuple(logits.shape)}, expected {shape}")
+        self.sample = policy.sample_actions(logits, self.rules, seed=self._seed, step=self._step.on(logits.device), rows=self._offset)
+        self._step.advance()
+        self.venv.stepAsync(self.sample.actions)
+
+
+class VecObservationDropout(VecEnvWrapper):
+    """Every feature of every observation is 0 with probability p, else divided by 1 - p (gym_amd.policy.dropout: p to 16 bits), for float32,
+    float16 and bfloat16 observations of any shape.  The observations are new tensors; what the venv returned stays as it was.
+
+    What is dropped for env i in the t-th observation since seed(s) follows from (seed, i's GLOBAL index, t) alone.  reset(index) has masks
+    of its own and leaves t as it is.  training = False passes the observations on untouched (t goes on all the same).
+    device_step=True keeps t on the GPU, for steps recorded into a graph."""
+
+    def __init__(self, venv: VecEnv, p: float, seed: int = 0, device_step: bool = False):
+        super().__init__(venv)
+        p = float(p)
+        if not 0.0 <= p < 1.0 or round(65536 * p) > 65535:
+            raise ValueError(f"p must lie in [0, 1) and round to less than 65536 / 65536, got {p}")
+        self.p, self.training = p, True
+        self._seed, self._step, self._offset = int(seed), _Counter(device_step), _env_offset(venv)
+
+    def seed(self, _seed):
+        self._seed = int(_seed)
+        self._step.restart()
+        return self.venv.seed(_seed)
+
+    def _drop(self, obs, rows, step):
+        from . import policy
+        n = obs.shape[0]
+        return policy.dropout(obs.reshape(n, -1), self.p, seed=self._seed, step=step, rows=rows).view(obs.shape)
+
+    def _next(self, obs):
+        step = self._step.on(obs.device)
+        if self.training:
+            obs = self._drop(obs, self._offset, step)
+        self._step.advance()
+        return obs
+
+    def reset(self, index=None):
+        if index is None:
+            return self._next(self.venv.reset())
+        obs = self.venv.reset(index)
+        # the number of the next observation, in the upper half of the steps' 48 bits, which the count does not reach
+        return self._drop(obs.unsqueeze(0), self._offset + int(index), self._step.on(obs.device) + (1 << 47)).squeeze(0) if self.training else obs
+
+    def stepWait(self):
+        r = self.venv.stepWait()
+        return r._replace(observation=self._next(r.observation))
 
 
 class Updater:

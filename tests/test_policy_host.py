@@ -187,3 +187,110 @@ def test_reference_generator_known_answers():
     assert abs(rate - 0.75) < 5 * (0.25 * 0.75 / 64000) ** 0.5
     u = R.uniforms(4000, 7)
     assert 0 < u.min() and u.max() < 1 and abs(u.mean().item() - 0.5) < 5 * (1 / 12 / 4000) ** 0.5
+
+
+# ---- the VecEnv wrappers' host side ------------------------------------------------------------------------------------------------------
+
+def fake_venv(n=4, a_space=None, offset=10):
+    from gym_amd import spaces
+    from gym_amd.vec_env import VecEnv, VecEnvStepReturn
+
+    class Fake(VecEnv):
+        env_offset = offset
+
+        def reset(self, index=None):
+            return torch.ones(n, 3) if index is None else torch.ones(3)
+
+        def stepAsync(self, actions):
+            self.actions = actions
+
+        def stepWait(self):
+            return VecEnvStepReturn(torch.ones(n, 3), torch.zeros(n, 1), torch.zeros(n, 1), [])
+
+        def seed(self, s):
+            return [s + i for i in range(n)]
+
+    o, a = spaces.cartpole_spaces()
+    return Fake(n, o, a_space or a)
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """Calls of the operators in place of the kernels."""
+    calls = []
+
+    def sample(logits, rules=None, *, seed, step=0, rows=0, out=None):
+        calls.append(("sample", seed, int(step), rows, rules))
+        return policy.ActionSample(torch.zeros(logits.shape[0], dtype=torch.int32), torch.zeros(logits.shape[0]))
+
+    def drop(x, p, *, seed, step=0, rows=0):
+        calls.append(("drop", seed, int(step), rows, tuple(x.shape)))
+        return x * 2
+
+    monkeypatch.setattr(policy, "sample_actions", sample)
+    monkeypatch.setattr(policy, "dropout", drop)
+    return calls
+
+
+@pytest.mark.parametrize("device_step", [False, True])
+def test_wrappers_key_their_draws_by_seed_global_row_and_step(recorded, device_step):
+    from gym_amd.vec_env import VecLogitActions, VecObservationDropout
+    inner = fake_venv()
+    venv = VecLogitActions(VecObservationDropout(inner, 0.25, seed=5, device_step=device_step), seed=6, device_step=device_step)
+    assert (venv.reset() == 2).all()
+    rules = policy.LogitRules(temperature=0.5)
+    for t in range(2):
+        r = venv.step(torch.zeros(4, 2))
+        assert (r.observation == 2).all() and inner.actions is venv.sample.actions
+        venv.rules = rules
+    assert (venv.reset(3) == 2).all() and venv.reset(3).shape == (3,)
+    assert recorded == [("drop", 5, 0, 10, (4, 3)), ("sample", 6, 0, 10, None), ("drop", 5, 1, 10, (4, 3)), ("sample", 6, 1, 10, rules),
+                        ("drop", 5, 2, 10, (4, 3)), ("drop", 5, 3 + (1 << 47), 13, (1, 3)), ("drop", 5, 3 + (1 << 47), 13, (1, 3))]
+    del recorded[:]
+    assert venv.seed(40) == [40, 41, 42, 43]   # the envs' seeds; the draws start again under the new one
+    venv.reset()
+    venv.venv.training = False
+    assert (venv.step(torch.zeros(4, 2)).observation == 1).all() and (venv.reset(0) == 1).all()
+    venv.venv.training = True
+    venv.step(torch.zeros(4, 2))
+    assert recorded == [("drop", 40, 0, 10, (4, 3)), ("sample", 40, 0, 10, rules), ("sample", 40, 1, 10, rules), ("drop", 40, 2, 10, (4, 3))]
+
+
+def test_wrappers_refuse(recorded):
+    from gym_amd import spaces
+    from gym_amd.vec_env import VecLogitActions, VecObservationDropout
+    with pytest.raises(TypeError, match="Discrete"):
+        VecLogitActions(fake_venv(a_space=spaces.makeBoxSpace(3)))
+    for p in (-0.1, 1.0, float("nan"), 1.0 - 2.0 ** -18):
+        with pytest.raises(ValueError, match="p must lie"):
+            VecObservationDropout(fake_venv(), p)
+    venv = VecLogitActions(fake_venv())
+    venv.reset()
+    for shape in ((4, 3), (3, 2), (4,), (4, 2, 1)):
+        with pytest.raises(ValueError, match="logits have shape"):
+            venv.step(torch.zeros(shape))
+    assert recorded == [] and venv.sample is None
+
+
+def test_wrappers_have_no_cpu_fallback():
+    from gym_amd.vec_env import VecLogitActions, VecObservationDropout
+    with pytest.raises(L.GymhipError, match="no CPU fallback"):
+        VecLogitActions(fake_venv()).step(torch.zeros(4, 2))
+    with pytest.raises(L.GymhipError, match="no CPU fallback"):
+        VecObservationDropout(fake_venv(), 0.5).reset()
+
+
+def test_binding_refuses_other_python_types():
+    for bad in (lambda: policy.process_logits([1.0]), lambda: policy.sample_actions(torch.zeros(2, 4), seed="a"), lambda: policy.dropout(torch.zeros(2, 4), 0.5, seed=1, step=None),
+                lambda: policy.LogitRules(mask=[1]), lambda: policy.LogitRules(temperature="hot")):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(ValueError, match="rules must be"):
+        policy.process_logits(torch.zeros(2, 4), {})
+    r = policy.LogitRules(temperature=0.5)
+    assert r.temperature == 0.5 and r.mask is None and r.repetition == 1.0
+    r.temperature = t = torch.ones(3)
+    assert r.temperature is t
+    r.temperature = -1.0   # assigned later, refused when used
+    with pytest.raises(ValueError, match="temperature"):
+        r._bind(torch.zeros(3, 4))
