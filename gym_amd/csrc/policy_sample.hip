@@ -190,15 +190,20 @@ __device__ inline int walk(const double* e, double s, double before, double leve
     return (first & (W - 1)) * C + at;
 }
 
-__device__ inline float log_prob_of(double y, double m, double k2, double sum) { return (float)(((y - m) * k2 - log2_double(sum)) * kLn2); }
-
-// A row's answer, by one lane: `at` its chosen column unless there is none.
+// A row's answer, by one lane: `at` its chosen column unless there is none, and that column's weight.  The logarithm of a weight by itself and the sum's
+// differ by 1e-16 of y: a column that is all of the sum has probability 1 for certain, and none has more.
 template <typename E>
 __device__ inline void answer(const Row& w, const typename E::T* x, const Mass& mass, int64_t at, uint32_t count, const Heat& c, int64_t b,
-                              int32_t* actions, float* log_prob) {
+                              int32_t* actions, float* log_prob, const double* chosen) {
     const bool none = mass.bad || mass.base == -INFINITY;
     actions[b] = none ? -1 : (int32_t)at;
-    log_prob[b] = mass.bad ? NAN : none ? -INFINITY : log_prob_of(ruled(w, (float)x[at], count, true, at), mass.base, c.k2, mass.sum);
+    float lp = mass.bad ? NAN : -INFINITY;
+    if (!none) {
+        const double y = ruled(w, (float)x[at], count, true, at) - mass.base;
+        const double share = chosen ? *chosen : weight(y, c);
+        lp = share >= mass.sum ? 0.0f : (float)__builtin_fmin((y * c.k2 - log2_double(mass.sum)) * kLn2, 0.0);
+    }
+    log_prob[b] = lp;
 }
 
 // Rows of at most G * C columns, G <= 64: one vector a lane, kBlock / G rows per workgroup.
@@ -237,7 +242,11 @@ __global__ void __launch_bounds__(kBlock) sample_vectors_kernel(const typename E
         }
         int64_t at = walk<G, C>(e, s, 0.0, row_uniform(keys, b) * mass.sum, mass.sum * 0x1p-80);
         if (w.greedy) at = first;
-        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? words[group * cap + at] : 0u, c, b, actions, log_prob);
+        double chosen = e[0];
+#pragma unroll
+        for (int j = 1; j < C; j++) chosen = at == j ? e[j] : chosen;
+        if (lane == 0 && own < rows)
+            answer<E>(w, x, mass, at, hist && at < width ? words[group * cap + at] : 0u, c, b, actions, log_prob, G == 1 ? &chosen : nullptr);
     }
 }
 
@@ -358,7 +367,7 @@ __global__ void __launch_bounds__(kBlock) sample_strips_kernel(const typename E:
             strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums[group]);
             at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums[group], &lds_at);
         }
-        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob);
+        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob, nullptr);
     }
 }
 
@@ -461,7 +470,7 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
             strip_sums<E, RULES, kBlock>(x, v, w, p, nv, scale, base, sums);
             at = lo + locate<E, RULES, kBlock>(x, w, p, nv, scale, base, parts_b[c].sum, target, sums, &lds_at);
         }
-        if (threadIdx.x == 0) answer<E>(w, x, mass, at, any && hist ? counts.at((int)(at % cap)) : 0u, scale, b, actions, log_prob);
+        if (threadIdx.x == 0) answer<E>(w, x, mass, at, any && hist ? counts.at((int)(at % cap)) : 0u, scale, b, actions, log_prob, nullptr);
         __syncthreads();
     }
 }

@@ -272,6 +272,24 @@ def test_greedy_takes_the_lowest_of_equal_ones(width):
     assert torch.equal(s.actions.cpu().long(), (x == x.max(1, keepdim=True).values).int().argmax(1))
 
 
+@pytest.mark.parametrize("width", [1, 2, 3, 8, 18, 100, 2049, 9001, 140001])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_no_probability_is_above_one(dtype, width):
+    """A choice that takes all of the weight has log-probability 0, not 1e-16 beside it; one that takes nearly all has nothing above 0."""
+    from gym_amd.policy import LogitRules, sample_actions
+    n = 64
+    g = torch.Generator().manual_seed(width)
+    at = torch.randint(0, width, (n,), generator=g)
+    alone = torch.full((n, width), -math.inf)
+    alone[torch.arange(n), at] = torch.randn(n, generator=g) * 30
+    s = sample_actions(alone.to(dtype).cuda(), LogitRules(temperature=0.7), seed=3)
+    assert torch.equal(s.actions.cpu().long(), at) and (s.log_prob == 0).all()
+    peaked = torch.randn(n, width, generator=g) * 3
+    peaked[torch.arange(n), at] += torch.linspace(5, 90, n)
+    for rules in (None, LogitRules(temperature=0.7)):
+        assert (check_sample(peaked.to(dtype).cuda(), rules, 3).log_prob <= 0).all()
+
+
 @pytest.mark.parametrize("width", [2, 3, 18, 200, 3001])
 def test_samples_follow_the_softmax(width):
     """Frequencies over rows that share their logits, against p, within 6 standard errors; flat, peaked and masked alike."""
