@@ -372,10 +372,9 @@ __device__ inline void ruled_cols(const Row& w, const Raw<E, C>& raw, uint32_t b
     for (int j = 0; j < C; j++) y[j] = bits >> j & 1 ? y[j] : -INFINITY;
 }
 
-// Counts the ids of columns [lo, lo + cap) in the histories of rows [b0, b0 + n), n a power of two.  By the
-// whole workgroup: every thread comes here, and counts may be read after it returns.  Integer LDS atomics, so their order is free.
+// Counts the ids of columns [lo, lo + span) of a row's history, `step` lanes together of which this one is `first`, from place `base` on.
 template <typename Id>
-__device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_t span, int first, int step, const Counts& c, int base) {
+__device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_t span, int first, int step, const Counts& c, int base, bool bits) {
     struct __attribute__((packed, aligned(sizeof(Id)))) Four { Id v[4]; };
     uint32_t* touched = c.touched();
     auto count = [&](Id id) {
@@ -384,10 +383,10 @@ __device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_
             const int at = base + (int)off;
             if (c.half) atomicAdd(&c.words[at >> 1], 1u << (16 * (at & 1)));
             else atomicAdd(&c.words[at], 1u);
-            if (c.bits) atomicOr(&touched[at >> 5], 1u << (at & 31));
+            if (bits) atomicOr(&touched[at >> 5], 1u << (at & 31));
         }
     };
-    for (int64_t i = (int64_t)first * 4; i < len; i += (int64_t)step * 4) {
+    for (int64_t i = (int64_t)first * 4; i < len; i += (int64_t)step * 4) {   // (2 or 4 loads under way: the same or, for their registers, slower)
         if (i + 4 <= len) {
             const Four f = *(const Four*)(ids + i);
 #pragma unroll
@@ -397,12 +396,23 @@ __device__ inline void count_row(const Id* ids, int64_t len, int64_t lo, uint32_
         }
     }
 }
+// Counts the ids of columns [lo, lo + cap) in the histories of rows [b0, b0 + n), n a power of two.  By the
+// whole workgroup: every thread comes here, and counts may be read after it returns.  Integer LDS atomics, so their order is free.  Lanes that add to one
+// word wait for each other, and ids repeat: where the row's columns leave most of its tile empty, adjacent lanes count in
+// copies, added up afterwards (1,339 rows of 3 columns after 12,191 ids: 178 -> 71 us).  COPIES false: rows wider than a tile, which leave nothing.
+template <bool COPIES = true>
 __device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows, int64_t width, int64_t lo, const Counts& c) {
     __syncthreads();
     for (int i = threadIdx.x; i < c.size() / 4; i += kBlock) ((uint4*)c.words)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const uint32_t span = (uint32_t)(lo + c.cap < width ? c.cap : width - lo);
     const int each = kBlock / n, mine = (int)threadIdx.x / each;   // `each` adjacent threads take a row
+    const int first = (int)threadIdx.x & (each - 1);
+    int pitch = c.cap, copies = 1;
+    while (COPIES && copies < each && copies < 16 && pitch % 4 == 0 && span * 2 <= (uint32_t)pitch) {
+        pitch /= 2;
+        copies *= 2;
+    }
     const int64_t b = b0 + mine;
     if (b < rows) {
         int64_t len = r.hist_cols;
@@ -410,11 +420,33 @@ __device__ inline void count_ids(const Rules& r, int64_t b0, int n, int64_t rows
             const int64_t have = r.len64 ? ((const int64_t*)r.hist_len)[b] : (int64_t)((const int32_t*)r.hist_len)[b];
             len = have < len ? have : len;
         }
-        const int first = (int)threadIdx.x & (each - 1);
-        if (r.hist64) count_row((const int64_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, mine * c.cap);
-        else count_row((const int32_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, mine * c.cap);
+        const int base = mine * c.cap + (first & (copies - 1)) * pitch;
+        const bool bits = c.bits && copies == 1;
+        if (r.hist64) count_row((const int64_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, base, bits);
+        else count_row((const int32_t*)r.hist + b * r.hist_stride, len, lo, span, first, each, c, base, bits);
     }
     __syncthreads();
+    if (copies > 1) {
+        // a word at a time (of 16-bit counts two, which no sum overflows): the copies' columns are cleared, nobody has them
+        const int shift = c.half ? 1 : 0, words = (int)(span + shift) >> shift;
+        for (int i = first; i < words; i += each) {
+            uint32_t* w = c.words + (mine * c.cap >> shift) + i;
+            uint32_t sum = w[0];
+            for (int k = 1; k < copies; k++) {
+                uint32_t* more = w + k * (pitch >> shift);
+                sum += *more;
+                *more = 0;
+            }
+            w[0] = sum;
+            if (c.bits) {
+                const int at = mine * c.cap + (i << shift);
+                const uint32_t low = c.half ? sum & 0xFFFFu : sum, high = c.half ? sum >> 16 : 0u;
+                const uint32_t set = (low ? 1u : 0u) | (high ? 2u : 0u);
+                if (set) atomicOr(&c.touched()[at >> 5], set << (at & 31));
+            }
+        }
+        __syncthreads();
+    }
 }
 
 // A workgroup's tile of columns is kTile 16-byte vectors a lane at most; half as many where the counts take 32 bits, so that both fit the same LDS.
@@ -422,6 +454,14 @@ constexpr int kTile = 4;
 template <typename E>
 constexpr int counts_words() { return kBlock * E::kVec * kTile / 2 + kBlock * E::kVec * kTile / 32; }
 inline bool half_counts(const Rules& r) { return r.hist_cols <= 65535; }
+
+// Lanes that share a row which `least` lanes hold: more of them where a history is to be counted and the rows alone do not make the 2,048 workgroups that
+// fill the chip (1,339 rows of 3 columns after 12,191 ids each, 256 lanes instead of one: 3,400 -> NNN us).
+inline int lanes_for(const Rules& r, int64_t rows, int least) {
+    int g = least;
+    while (g < kBlock && r.hist && r.hist_cols > 4 * g && rows * g < 2048 * kBlock) g *= 2;
+    return g;
+}
 
 // ---- reductions over G lanes: G <= 64 adjacent lanes of a wave by lane permutations in the vector unit, G = kBlock through LDS as well --------
 template <int CTRL, int ROWS = 0xF>

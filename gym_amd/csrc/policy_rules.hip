@@ -21,6 +21,7 @@ Tiling tiling(int64_t rows, int64_t width, const Rules& r) {
     t.half = half_counts(r);
     t.lanes_log2 = 0;
     while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) < width) t.lanes_log2++;
+    for (const int lanes = lanes_for(r, rows, 1 << t.lanes_log2); 1 << t.lanes_log2 < lanes;) t.lanes_log2++;
     const int64_t step = (int64_t)E::kVec << t.lanes_log2;
     const int64_t need = (width + step - 1) / step, most = r.hist && !t.half ? kTile / 2 : kTile;
     t.nv = (int)(need < most ? need : most);

@@ -250,7 +250,37 @@ __global__ void __launch_bounds__(kBlock) sample_vectors_kernel(const typename E
     }
 }
 
-// A strip of a row: the columns of G = 64 or kBlock lanes, nv <= kTile vectors each, gone through one vector at a time with the next one's load
+// Where the running sum of n parts passes `level`, 64 parts at a time, by each wave for itself: the part, or the last one with more than `tiny` should
+// rounding leave the level above all sums (*past); *before: what comes before it.
+template <typename F>
+__device__ inline int64_t find_part(int64_t n, double level, double tiny, F part_sum, double* before, bool* past) {
+    const int lane = (int)threadIdx.x & (kWave - 1);
+    int64_t last = 0;
+    double run = 0;
+    for (int64_t c0 = 0; c0 < n; c0 += kWave) {
+        const double e = c0 + lane < n ? part_sum(c0 + lane) : 0.0;
+        const double upto = running_sum<kWave>(e, lane);
+        const uint64_t hits = __ballot(e > 0 && run + upto > level), some = __ballot(e > tiny);
+        if (hits) {
+            const int at = __ffsll((unsigned long long)hits) - 1;
+            *before = run + __shfl(upto - e, at);
+            *past = false;
+            return c0 + at;
+        }
+        if (some) last = c0 + 63 - __clzll((long long)some);
+        run += __shfl(upto, kWave - 1);
+    }
+    *before = 0;
+    *past = true;
+    return last;
+}
+
+// Vectors a lane in a strip of a wave without a history, at most (a workgroup's: a quarter), and where which is taken.  Rows of a wave each are done in fewer
+// instructions, a workgroup a row has four times the waves for few rows, parts and a join sixteen times.  Measured, us, wave / workgroup / parts:
+// bf16 8192 x 2,083: 26 / 48 / -; f32 8192 x 4,097: 38 / 72 / 117; f32 512 x 16,384: 34 / 14 / 20; bf16 64 x 32,768: 44 / 14.5 / 12.8.
+constexpr int kLong = 256;
+
+// A strip of a row: the columns of G = 64 or kBlock lanes, nv vectors each, gone through one vector at a time with the next one's load
 // under way: few registers, so that many waves are there to wait for memory and for the workgroup's barriers.
 template <typename E, typename F>
 __device__ inline void each_vector(const Row& w, const typename E::T* x, const Place& p, int nv, Vector<E, E::kVec> next, F f) {
@@ -278,17 +308,34 @@ __device__ inline void strip_sums(const typename E::T* x, const Vector<E, E::kVe
     group_sync<G>();
 }
 
-// The sum of a strip.
-template <typename E, bool RULES, int G>
+// The sum of a strip.  KEEP: and against 0 what strip_sums would leave, *kept; else that pass is still to be made.
+template <typename E, bool RULES, int G, bool KEEP>
 __device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec>& v0, const Row& w, const Place& p, int nv, const Heat& c, double* lds,
-                                 long long* first) {
-    constexpr int C = E::kVec;
+                                 long long* first, double* sums, bool* kept) {
+    constexpr int C = E::kVec, M = G / kWave;
+    if (KEEP) *kept = false;
     if (!w.greedy) {   // one row's: all lanes alike
         double sum = 0;
         uint64_t beyond = 0;
-        each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) { sum += weigh_apart<E, RULES>(w, p, k, v, c, &beyond); });
-        const Mass mass{0.0, group_reduce<G>(mine_in(beyond) ? (double)NAN : sum, Sum<double>(), lds), false};
-        if (mass.sum > 0x1p-900) return mass;
+        if constexpr (KEEP) {
+            const int wave = G > kWave ? (int)threadIdx.x / kWave : 0;
+            group_sync<G>();
+            each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) {
+                double s = weigh_apart<E, RULES>(w, p, k, v, c, &beyond);
+                s = group_reduce<kWave>(mine_in(beyond) ? (double)NAN : s, Sum<double>(), (double*)nullptr);
+                if ((threadIdx.x & (kWave - 1)) == 0) sums[k * M + wave] = s;
+                sum += s;
+            });
+            if (G > kWave) sum = group_reduce<G>((threadIdx.x & (kWave - 1)) == 0 ? sum : 0.0, Sum<double>(), lds);
+            group_sync<G>();
+        } else {
+            each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) { sum += weigh_apart<E, RULES>(w, p, k, v, c, &beyond); });
+            sum = group_reduce<G>(mine_in(beyond) ? (double)NAN : sum, Sum<double>(), lds);
+        }
+        if (sum > 0x1p-900) {
+            if (KEEP) *kept = true;
+            return Mass{0.0, sum, false};
+        }
     }
     return sum_against_max<E, RULES, G, C>(x, w, p, nv, c, lds, first);
 }
@@ -301,24 +348,10 @@ __device__ inline int locate(const typename E::T* x, const Row& w, const Place& 
     constexpr int C = E::kVec, M = G / kWave;
     const int wave = G > kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave) : 0;
     const double tiny = sum * 0x1p-80;
-    // the part (vector, wave) that holds the level, and what comes before it
-    int part = -1, some = 0;
-    double before = 0;
-#pragma unroll 1
-    for (int i = 0; i < nv * M; i++) {
-        if (before + sums[i] > level) {
-            part = i;
-            break;
-        }
-        before += sums[i];
-        if (sums[i] > tiny) some = i;
-    }
-    if (part < 0) {
-        part = some;
-        before = 0;
-        level = INFINITY;
-    }
-    part = __builtin_amdgcn_readfirstlane(part);
+    double before;
+    bool past;
+    const int part = __builtin_amdgcn_readfirstlane((int)find_part(nv * M, level, tiny, [&](int64_t i) { return sums[i]; }, &before, &past));   // (vector, wave)
+    if (past) level = INFINITY;
     const int k = part / M, at_wave = part - k * M;
     int column = 0;
     if (wave == at_wave) {
@@ -341,10 +374,10 @@ __device__ inline int locate(const typename E::T* x, const Row& w, const Place& 
 template <typename E, bool RULES, int G>
 __global__ void __launch_bounds__(kBlock) sample_strips_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
                                                                int nv, bool half, int32_t* actions, float* log_prob) {
-    constexpr int C = E::kVec, per = kBlock / G, M = G / kWave;
+    constexpr int C = E::kVec, per = kBlock / G;
     __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
     __shared__ double lds[kBlock / kWave];
-    __shared__ double sums[per][kTile * M];
+    __shared__ double sums[per][kLong];
     __shared__ int lds_at;
     const int cap = G * C * nv;
     const int lane = (int)threadIdx.x & (G - 1), group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : 0;
@@ -361,10 +394,11 @@ __global__ void __launch_bounds__(kBlock) sample_strips_kernel(const typename E:
         if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
         const Heat c = w;
         long long first = 0;
-        const Mass mass = sum_strip<E, RULES, G>(x, v, w, p, nv, c, lds, &first);
+        bool kept;
+        const Mass mass = sum_strip<E, RULES, G, true>(x, v, w, p, nv, c, lds, &first, sums[group], &kept);
         int64_t at = first;
         if (!w.greedy && !mass.bad && mass.base > -INFINITY) {   // the group's lanes alike
-            strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums[group]);
+            if (!kept) strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums[group]);
             at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums[group], &lds_at);
         }
         if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob, nullptr);
@@ -394,9 +428,9 @@ __global__ void __launch_bounds__(kBlock) sample_parts_kernel(const typename E::
         const typename E::T* x = x0 + b * stride;
         Vector<E, C> v;
         v.load(w, x, p.at, width);
-        if (hist) count_ids(r, b, 1, rows, width, lo, counts);
+        if (hist) count_ids<false>(r, b, 1, rows, width, lo, counts);
         long long first = 0;
-        const Mass mass = sum_strip<E, RULES, kBlock>(x, v, w, p, nv, w, lds, &first);
+        const Mass mass = sum_strip<E, RULES, kBlock, false>(x, v, w, p, nv, w, lds, &first, nullptr, nullptr);
         if (threadIdx.x == 0) parts[b * cuts + blockIdx.x] = Part{mass.base, mass.bad ? (double)NAN : mass.base == -INFINITY ? 0.0 : mass.sum, first};
     }
 }
@@ -429,7 +463,7 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
         bad = group_reduce<kWave>(bad, Max<int>(), (int*)none);
         const bool any = !bad && m > -INFINITY;   // the same for the whole workgroup, as is what hangs on it
         // a part's sum against m
-        auto share = [&](int64_t c) { return c < cuts && parts_b[c].sum > 0 ? parts_b[c].sum * weight(parts_b[c].base - m, scale) : 0.0; };
+        auto share = [&](int64_t c) { return parts_b[c].sum > 0 ? parts_b[c].sum * weight(parts_b[c].base - m, scale) : 0.0; };
         double sum = 0;
         long long first = width;
         if (any)
@@ -441,32 +475,19 @@ __global__ void __launch_bounds__(kBlock) sample_join_kernel(const typename E::T
         int64_t at = 0;
         if (any && w.greedy) {
             at = group_reduce<kWave>(first, Min<long long>(), (long long*)none);
-            if (hist) count_ids(r, b, 1, rows, width, at / cap * cap, counts);
+            if (hist) count_ids<false>(r, b, 1, rows, width, at / cap * cap, counts);
         } else if (any) {
             const double level = u * mass.sum, tiny = mass.sum * 0x1p-80;
-            int64_t part = -1, last = 0;   // last: the last part with any weight, should rounding leave the level above all sums
-            double run = 0, before = 0;
-            for (int64_t c0 = 0; c0 < cuts && part < 0; c0 += kWave) {
-                const double e = share(c0 + lane);
-                const double upto = running_sum<kWave>(e, lane);
-                const uint64_t hits = __ballot(e > 0 && run + upto > level), some = __ballot(e > tiny);
-                if (hits) {
-                    const int at_lane = __ffsll((unsigned long long)hits) - 1;
-                    part = c0 + at_lane;
-                    before = run + __shfl(upto - e, at_lane);
-                } else if (some) {
-                    last = c0 + 63 - __clzll((long long)some);
-                }
-                run += __shfl(upto, kWave - 1);
-            }
-            const int64_t c = part < 0 ? last : part;
+            double before;
+            bool past;
+            const int64_t c = find_part(cuts, level, tiny, share, &before, &past);
             const double base = parts_b[c].base;
-            const double target = part < 0 ? INFINITY : (level - before) / weight(base - m, scale);
+            const double target = past ? INFINITY : (level - before) / weight(base - m, scale);
             const int64_t lo = c * cap;
             const Place p{lo + place, width, kBlock * C, place, counts};
             Vector<E, C> v;
             v.load(w, x, p.at, width);
-            if (hist) count_ids(r, b, 1, rows, width, lo, counts);
+            if (hist) count_ids<false>(r, b, 1, rows, width, lo, counts);
             strip_sums<E, RULES, kBlock>(x, v, w, p, nv, scale, base, sums);
             at = lo + locate<E, RULES, kBlock>(x, w, p, nv, scale, base, parts_b[c].sum, target, sums, &lds_at);
         }
@@ -535,17 +556,23 @@ struct Launch {
         const int most = strip_vectors(r);
         const auto need = [&](int g) { return (int)((width + g * v - 1) / (g * v)); };   // vectors a lane
         // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then strips
-        if (width <= 2) vectors<1, 2>();
-        else if (width <= 4) vectors<1, 4>();
-        else if (width <= v) vectors<1, v>();
-        else if (width <= 2 * v) vectors<2, v>();
-        else if (width <= 4 * v) vectors<4, v>();
-        else if (width <= 8 * v) vectors<8, v>();
-        else if (width <= 16 * v) vectors<16, v>();
-        else if (width <= 32 * v) vectors<32, v>();
-        else if (width <= 64 * v) vectors<64, v>();
-        else if (width <= 64 * v * most) strips<64>(need(64));
-        else if (width <= (int64_t)kBlock * v * most) strips<kBlock>(need(kBlock));
+        int g = 1;
+        while (g < kWave && width > g * v) g *= 2;
+        g = lanes_for(r, rows, g);
+        if (width <= kWave * v && g <= kWave) {
+            if (g == 1 && width <= 2) vectors<1, 2>();
+            else if (g == 1 && width <= 4) vectors<1, 4>();
+            else if (g == 1) vectors<1, v>();
+            else if (g == 2) vectors<2, v>();
+            else if (g == 4) vectors<4, v>();
+            else if (g == 8) vectors<8, v>();
+            else if (g == 16) vectors<16, v>();
+            else if (g == 32) vectors<32, v>();
+            else vectors<64, v>();
+        }
+        else if (width <= kWave * v * most && g <= kWave) strips<kWave>(need(kWave));
+        else if (!r.hist && need(kWave) <= kLong && rows >= 128 * need(kWave)) strips<kWave>(need(kWave));
+        else if (need(kBlock) <= most || (!r.hist && need(kBlock) <= kLong / 4 && (need(kBlock) <= 8 || rows >= 16 * need(kBlock)))) strips<kBlock>(need(kBlock));
         else wide(wide_nv(v, most, rows, width));
     }
 };

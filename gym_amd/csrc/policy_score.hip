@@ -1,150 +1,132 @@
 // policy_score.hip — log-probability and entropy of given actions under the ruled logits: one pass over the logits with a running maximum.
 //
-// With y the logit after penalties and bias, d = y - max y, t = d log2 e / T and w = 2^t:  S = sum w, D = sum w t,
-// log_prob = d_a / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to d, not to y); a lane adds up
-// at most 32 of them before it goes on in double.
+// With y the logit after penalties and bias, m a float about the greatest y, t = (y - m) log2 e / T and w = 2^t:  S = sum w, D = sum w t,
+// log_prob = (y_a - m) / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to y - m, not to y); a lane adds up
+// at most 32 of them before it goes on in double.  m is the same for a wave, so that the sums hardly ever have to be brought to a new one: a few times in
+// a row, by the logarithm of its length.  8.5 vector instructions a column, of the 16 that 2-byte logits leave time for at the memory's rate.
 #include "policy_common.h"
 
 namespace gymhip {
 namespace policy {
 namespace {
 
-// A running (m, S, D) over any set of columns; S and D against m.
+// A running (m, S, D) over any set of columns, S and D against m.  A NaN or +inf among them makes S NaN; m = -inf: nothing yet.
 struct Run {
-    double m, s, d;
-    int bad;
+    float m;
+    double s, d;
 };
 
-// S and D of r against another base m >= r.m.
-__device__ inline void rebase(Run& r, double m, double k2) {
-    if (r.m == m || r.s == 0) { r.m = m; return; }
-    const double t = (r.m - m) * k2;
-    const double e = (double)__builtin_amdgcn_exp2f((float)t);
-    // against the new base every t moves by the same amount
-    r.d = e == 0 ? 0.0 : e * (r.d + t * r.s);
-    r.s = e * r.s;
+// S and D of r against another base m > r.m.
+__device__ inline void rebase(Run& r, float m, double k2) {
+    if (r.m > -INFINITY && r.m < m) {
+        double t = ((double)r.m - (double)m) * k2;
+        t = t > -200 ? t : -200;   // 0 at float32's precision
+        const double e = exp2_double(t, 1.0);
+        r.d = e * __builtin_fma(t, r.s, r.d);   // against the new base every t moves by the same amount
+        r.s = e * r.s;
+    }
     r.m = m;
 }
 
-// N columns' y added to a run.  NaN and +inf only mark it.
+// w = 2^t and w t of one column added to s and d.  A NaN gets through by w; where w is 0 (2^-200 is, in float32) t is kept finite.
+__device__ inline void add_term(float t, float& s, float& d) {
+    const float w = __builtin_amdgcn_exp2f(t);
+    s += w;
+    d = __builtin_fmaf(w, __builtin_fmaxf(t, -200.f), d);
+}
+__device__ inline float gap(float y, float m) { return y - m; }
+__device__ inline float gap(double y, float m) { return (float)(y - (double)m); }
+
+// N columns' y of every lane of the wave added to the lanes' runs, whose m is the wave's.
 template <int N, typename Y>
 __device__ inline void add_cols(Run& run, const Y* y, double k2) {
-    Y m = -INFINITY;
-    bool bad = false;
+    float top = (float)y[0];
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        bad = bad || y[j] != y[j];
-        m = y[j] > m ? y[j] : m;
+    for (int j = 1; j < N; j++) top = __builtin_fmaxf(top, (float)y[j]);
+    if (__any(!(top <= run.m))) rebase(run, group_reduce<kWave>(__builtin_fmaxf(top, run.m), Max<float>(), (float*)nullptr), k2);
+    if (run.m == -INFINITY) {
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < N; j++) nan = nan || y[j] != y[j];
+        if (nan) run.s = NAN;
+        return;
     }
-    if (bad || m == INFINITY) run.bad = 1;
-    if (!(m > -INFINITY && m < INFINITY)) return;
-    if ((double)m > run.m) rebase(run, (double)m, k2);
-    const float k = (float)k2;
+    const float k = (float)k2, m = run.m;
     float s = 0, d = 0;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        // y - m where m is a float too is exact to a half step as a float; against an earlier base, which may not be one, it is taken in double
-        const float gap = sizeof(Y) == 4 && N > 8 ? (float)(y[j] - m) : (float)((double)y[j] - run.m);
-        float t = gap * k;
-        t = t > -200.f ? t : -200.f;   // 2^-200 is 0 in float32; keeps 0 * inf out
-        const float w = __builtin_amdgcn_exp2f(t);
-        s += w;
-        d = __builtin_fmaf(w, t, d);
-    }
-    if (sizeof(Y) == 4 && N > 8) {   // against the columns' own maximum: brought to the run's
-        Run more{(double)m, (double)s, (double)d, 0};
-        rebase(more, run.m, k2);
-        run.s += more.s;
-        run.d += more.d;
-    } else {
-        run.s += (double)s;
-        run.d += (double)d;
-    }
+    for (int j = 0; j < N; j++) add_term(gap(y[j], m) * k, s, d);
+    run.s += (double)s;
+    run.d += (double)d;
 }
 
-// A lane's columns: nv vectors from `at` on, `step` columns apart, added to its run; `place` is the first's place in the counts.  Logits without
-// rules (NV vectors) are loaded first, all of them, and summed together; else it goes a vector at a time, the next one's load under way, in double
-// where a bias, or a count in any of the wave's lanes, makes y differ from the logits.  count() makes the counts while the first load is under
-// way.
-template <typename E, bool RULES, int NV, int C, typename Count>
+// A lane's columns: nv vectors from `first` on, `step` columns apart, added to its run, one at a time with the next one's load under way; `place` is the first's
+// place in the counts.  count() makes the counts while the first load is under way.
+template <typename E, bool RULES, typename Count>
 __device__ inline void add_columns(Run& run, const Row& w, const typename E::T* x, int64_t first, int step, int nv, int64_t width, const Counts& counts, int place,
                                    double k2, Count count) {
-    if constexpr (RULES) {
-        Vector<E, C> next;
-        next.load(w, x, first, width);
-        count();
+    constexpr int C = E::kVec;
+    Vector<E, C> next;
+    next.load(w, x, first, width);
+    count();
 #pragma unroll 1
-        for (int k = 0; k < nv; k++) {
-            const int64_t at = first + k * step;
-            Vector<E, C> v = next;
-            if (k + 1 < nv) next.load(w, x, at + step, width);
-            if (at >= width) continue;
-            if constexpr (NV == 1) {   // narrow rows: all columns alike
-                double y[C];
-                ruled_cols(w, v.raw, v.bits, at, width, counts, place, counts.words != nullptr, y);
-                add_cols<C>(run, y, k2);
-            } else {
-                // the few columns with a count are left out of the straight pass, and each is added by itself by the lane that owns it
-                uint32_t apart = counts.words ? counts.which<C>(place + k * step) & v.bits : 0u;
-                const Raw<E, C> whole = v.raw;
-                if (w.masked || __any(apart)) v.raw.keep(v.bits & ~apart);
-                if (w.biased) {
-                    float f[C];
-                    double y[C];
-                    bias_cols<C>(w, at, width, f);
+    for (int k = 0; k < nv; k++) {
+        const int64_t at = first + (int64_t)k * step;
+        Vector<E, C> v = next;
+        if (k + 1 < nv) next.load(w, x, at + step, width);
+        // the few columns with a count are left out of the straight pass, and each is added by itself by the lane that owns it
+        uint32_t apart = RULES && counts.words ? counts.which<C>(place + k * step) & v.bits : 0u;
+        const Raw<E, C> whole = v.raw;
+        if (w.masked || (RULES && __any(apart))) v.raw.keep(v.bits & ~apart);
+        if (RULES && w.biased) {
+            float f[C];
+            double y[C];
+            bias_cols<C>(w, at, width, f);
 #pragma unroll
-                    for (int j = 0; j < C; j++) y[j] = (double)v.raw.get(j) + (double)f[j];
-                    if (w.masked) {   // whatever the bias is there
+            for (int j = 0; j < C; j++) y[j] = (double)v.raw.get(j) + (double)f[j];
+            if (w.masked) {   // whatever the bias is there
 #pragma unroll
-                        for (int j = 0; j < C; j++) y[j] = v.bits >> j & 1 ? y[j] : -INFINITY;
-                    }
-                    add_cols<C>(run, y, k2);
-                } else {
-                    float y[C];
+                for (int j = 0; j < C; j++) y[j] = v.bits >> j & 1 ? y[j] : -INFINITY;
+            }
+            add_cols<C>(run, y, k2);
+        } else {
+            float y[C];
 #pragma unroll
-                    for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
-                    add_cols<C>(run, y, k2);
-                }
-                while (apart) {
-                    const int j = __ffs((int)apart) - 1;
-                    apart &= apart - 1;
-                    const double y = ruled(w, whole.pick(j), counts.at(place + k * step + j), true, at + j);
-                    add_cols<1>(run, &y, k2);
-                }
+            for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
+            add_cols<C>(run, y, k2);
+        }
+        if constexpr (RULES) {
+            while (__any(apart)) {   // lanes without one add nothing
+                const int j = __ffs((int)apart) - 1;
+                const double y = apart ? ruled(w, whole.pick(j < 0 ? 0 : j), counts.at(place + k * step + (j < 0 ? 0 : j)), true, at + j) : -(double)INFINITY;
+                apart &= apart - 1;
+                add_cols<1>(run, &y, k2);
             }
         }
-    } else {
-        Raw<E, C> raw[NV];
-        uint32_t bits[NV];
-#pragma unroll
-        for (int k = 0; k < NV; k++) raw[k].load(x, first + k * step, NV == 1 || first + k * step < width ? width : 0);
-        if (w.masked) {
-#pragma unroll
-            for (int k = 0; k < NV; k++) bits[k] = allowed_bits(w, first + k * step, width);
-        }
-        float y[NV * C];
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            if (w.masked) raw[k].keep(bits[k]);
-#pragma unroll
-            for (int j = 0; j < C; j++) y[k * C + j] = raw[k].get(j);
-        }
-        add_cols<NV * C>(run, y, k2);
     }
 }
 
-// The group's run from its lanes'.
+// The group's run from its lanes': the waves', each against its m, and for a workgroup these.
 template <int G>
-__device__ inline void join(Run& run, double k2, double* lds) {
-    const double m = group_reduce<G>(run.m, Max<double>(), lds);
-    run.bad = group_reduce<G>(run.bad, Max<int>(), (int*)lds);
-    if (m > -INFINITY) rebase(run, m, k2);
-    run.s = group_reduce<G>(run.s, Sum<double>(), lds);
-    run.d = group_reduce<G>(run.d, Sum<double>(), lds);
+__device__ inline void join(Run& run, double k2, Run* lds) {
+    run.s = group_reduce<kWave>(run.s, Sum<double>(), (double*)nullptr);
+    run.d = group_reduce<kWave>(run.d, Sum<double>(), (double*)nullptr);
+    if (G == kWave) return;
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = run;
+    __syncthreads();
+    float m = lds[0].m;
+    for (int i = 1; i < kBlock / kWave; i++) m = __builtin_fmaxf(m, lds[i].m);
+    run = Run{m, 0, 0};
+    for (int i = 0; i < kBlock / kWave; i++) {
+        Run one = lds[i];
+        rebase(one, m, k2);
+        run.s += one.s;
+        run.d += one.d;
+    }
 }
 
 __device__ inline void finish(const Run& run, const Row& w, double ya, int64_t b, float* log_prob, float* entropy, double* log_sum) {
-    if (run.bad) {
+    if (run.s != run.s) {
         log_prob[b] = NAN;
         entropy[b] = NAN;
         log_sum[2 * b] = 0;
@@ -152,10 +134,12 @@ __device__ inline void finish(const Run& run, const Row& w, double ya, int64_t b
         return;
     }
     const bool empty = run.m == -INFINITY;
-    const double ls = empty ? 0.0 : log(run.s);
-    log_prob[b] = empty ? -INFINITY : (float)((ya - run.m) / w.temp - ls);
-    entropy[b] = empty ? 0.f : (float)(ls - kLn2 * (run.d / run.s));
-    log_sum[2 * b] = empty ? 0.0 : run.m;   // apart: beside a mask of the type's lowest value the sum of the two would lose log S
+    const double l2 = empty ? 0.0 : log2_double(run.s), ls = l2 * kLn2;
+    double inv = empty ? 0.0 : __builtin_amdgcn_rcp(run.s);   // and a Newton step: 1e-14 of it
+    inv = __builtin_fma(__builtin_fma(-run.s, inv, 1.0), inv, inv);
+    log_prob[b] = empty ? -INFINITY : (float)(((ya - (double)run.m) * w.k2 - l2) * kLn2);
+    entropy[b] = empty ? 0.f : (float)((l2 - run.d * inv) * kLn2);
+    log_sum[2 * b] = empty ? 0.0 : (double)run.m;   // apart: beside a mask of the type's lowest value the sum of the two would lose log S
     log_sum[2 * b + 1] = empty ? -INFINITY : ls;
 }
 
@@ -170,33 +154,99 @@ __device__ inline double y_at(const Row& w, const typename E::T* x, int64_t widt
     return ruled(w, (float)x[v], count, allowed(w, v), v);
 }
 
-// Rows in the registers of G lanes, of NV vectors each at most (nv: as many as the row has).
-template <typename E, bool RULES, int G, int NV, int C>
-__global__ void __launch_bounds__(kBlock) score_rows_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int nv, bool half,
-                                                            const void* actions, int act64, float* log_prob, float* entropy, double* log_sum) {
-    constexpr int per = kBlock / G;
-    __shared__ __align__(16) uint32_t words[!RULES ? 4 : NV > 1 ? counts_words<E>() : kBlock * C];
-    __shared__ double lds[kBlock / kWave];
-    const int cap = G * C * nv;
+// The run of a group whose lanes hold all of its columns, C each: the greatest first, the sums against it.
+template <int G, int C, typename Y>
+__device__ inline Run run_of(const Y* y, double k2) {
+    float m = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        bad = bad || !(y[j] < (Y)INFINITY);
+        m = __builtin_fmaxf(m, (float)y[j]);
+    }
+    m = group_reduce<G>(bad ? (float)INFINITY : m, Max<float>(), (float*)nullptr);
+    if (m == INFINITY) return Run{m, NAN, 0};
+    if (m == -INFINITY) return Run{m, 0, 0};
+    const float k = (float)k2;
+    float s = 0, d = 0;
+#pragma unroll
+    for (int j = 0; j < C; j++) add_term(gap(y[j], m) * k, s, d);
+    return Run{m, (double)group_reduce<G>(s, Sum<float>(), (float*)nullptr), (double)group_reduce<G>(d, Sum<float>(), (float*)nullptr)};
+}
+
+// The action of a row and its logit, read early: both are on their way while the row is summed.
+template <typename E>
+struct Chosen {
+    int64_t a;
+    float x;
+    bool inside, open;
+    __device__ Chosen(const Row& w, const typename E::T* row, int64_t width, const void* actions, int act64, int64_t b) {
+        a = action_of(actions, act64, b);
+        inside = a >= 0 && a < width;
+        x = inside ? (float)row[a] : 0.f;
+        open = inside && allowed(w, a);
+    }
+    __device__ double y(const Row& w, uint32_t count) const { return open ? ruled(w, x, count, true, a) : -INFINITY; }
+};
+
+// Rows in the registers of G <= 64 lanes, a vector each.  Bound by the vector unit: what it takes to join and finish a row.
+template <typename E, bool RULES, int G, int C>
+__global__ void __launch_bounds__(kBlock) score_rows_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, const void* actions,
+                                                            int act64, float* log_prob, float* entropy, double* log_sum) {
+    constexpr int per = kBlock / G, cap = G * C;
+    __shared__ __align__(16) uint32_t words[RULES ? per * cap : 4];
     const int lane = (int)threadIdx.x & (G - 1);
     const int group = G >= kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : (int)threadIdx.x / G;
     const bool hist = RULES && r.hist;
-    const Counts counts{hist ? words : nullptr, cap, per * cap, NV > 1 && half, NV > 1};
+    const Counts counts{hist ? words : nullptr, cap, per * cap, false, false};
     for (int64_t band = blockIdx.x; band * per < rows; band += gridDim.x) {
         const int64_t own = band * per + group;
         const int64_t b = own < rows ? own : rows - 1;   // lanes without a row follow the last one: every exchange has all its lanes
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const double k2 = w.k2;
-        Run run{-INFINITY, 0, 0, 0};
-        add_columns<E, RULES, NV, C>(run, w, x, lane * C, G * C, nv, width, counts, group * cap + lane * C, k2, [&] {
+        Vector<E, C> v;
+        v.load(w, x, lane * C, width);
+        const Chosen<E> chosen(w, x, width, actions, act64, b);
+        Run run;
+        if (RULES && (hist || w.biased)) {
+            if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
+            double y[C];
+            ruled_cols(w, v.raw, v.bits, lane * C, width, counts, group * cap + lane * C, hist, y);
+            run = run_of<G, C>(y, w.k2);
+        } else {
+            if (w.masked) v.raw.keep(v.bits);
+            float y[C];
+#pragma unroll
+            for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
+            run = run_of<G, C>(y, w.k2);
+        }
+        if (lane == 0 && own < rows) finish(run, w, chosen.y(w, hist && chosen.inside ? counts.at(group * cap + (int)chosen.a) : 0u), b, log_prob, entropy, log_sum);
+    }
+}
+
+// Longer rows, by a wave each (G = 64) or a workgroup; under a history nv vectors are a tile, which holds the row.
+template <typename E, bool RULES, int G>
+__global__ void __launch_bounds__(kBlock) score_strips_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int nv, bool half,
+                                                              const void* actions, int act64, float* log_prob, float* entropy, double* log_sum) {
+    constexpr int C = E::kVec, per = kBlock / G;
+    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ Run lds[kBlock / kWave];
+    const int cap = G * C * nv;
+    const int lane = (int)threadIdx.x & (G - 1), group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : 0;
+    const bool hist = RULES && r.hist;
+    const Counts counts{hist ? words : nullptr, cap, per * cap, half, true};
+    for (int64_t band = blockIdx.x; band * per < rows; band += gridDim.x) {
+        const int64_t own = band * per + group;
+        const int64_t b = own < rows ? own : rows - 1;
+        const Row w = row_of<RULES>(r, b);
+        const typename E::T* x = x0 + b * stride;
+        const Chosen<E> chosen(w, x, width, actions, act64, b);
+        Run run{-INFINITY, 0, 0};
+        add_columns<E, RULES>(run, w, x, lane * C, G * C, nv, width, counts, group * cap + lane * C, w.k2, [&] {
             if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
         });
-        join<G>(run, k2, lds);
-        if (lane == 0 && own < rows) {
-            const int64_t a = action_of(actions, act64, b);
-            finish(run, w, y_at<E>(w, x, width, a, hist && a >= 0 && a < width ? counts.at(group * cap + (int)a) : 0u), b, log_prob, entropy, log_sum);
-        }
+        join<G>(run, w.k2, lds);
+        if (lane == 0 && own < rows) finish(run, w, chosen.y(w, hist && chosen.inside ? counts.at(group * cap + (int)chosen.a) : 0u), b, log_prob, entropy, log_sum);
     }
 }
 
@@ -213,8 +263,7 @@ __global__ void __launch_bounds__(kBlock) score_wide_kernel(const typename E::T*
                                                             float* entropy, double* log_sum, Part* parts) {
     constexpr int C = E::kVec;
     __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
-    __shared__ double lds[kBlock / kWave];
-    __shared__ double the_ya;
+    __shared__ Run lds[kBlock / kWave];
     const int cap = kBlock * C * nv, place = (int)threadIdx.x * C;
     const bool hist = RULES && r.hist;
     const Counts counts{hist ? words : nullptr, cap, cap, half, true};
@@ -224,21 +273,22 @@ __global__ void __launch_bounds__(kBlock) score_wide_kernel(const typename E::T*
         const int64_t c0 = part * each, c1 = c0 + each < cuts ? c0 + each : cuts;
         const Row w = row_of<RULES>(r, b);
         const typename E::T* x = x0 + b * stride;
-        const double k2 = w.k2;
-        const int64_t a = action_of(actions, act64, b);
-        Run run{-INFINITY, 0, 0, 0};
-        if (threadIdx.x == 0) the_ya = -INFINITY;
-        for (int64_t c = c0; c < c1; c++) {
-            const int64_t lo = c * cap;
-            add_columns<E, RULES, kTile, C>(run, w, x, lo + place, kBlock * C, nv, width, counts, place, k2, [&] {
-                if (hist) count_ids(r, b, 1, rows, width, lo, counts);
-            });
-            if (threadIdx.x == 0 && a >= lo && a < lo + cap) the_ya = y_at<E>(w, x, width, a, hist && a < width ? counts.at((int)(a - lo)) : 0u);
+        const Chosen<E> chosen(w, x, width, actions, act64, b);
+        Run run{-INFINITY, 0, 0};
+        double ya = chosen.y(w, 0u);
+        if (hist) {
+            for (int64_t c = c0; c < c1; c++) {
+                const int64_t lo = c * cap;
+                add_columns<E, RULES>(run, w, x, lo + place, kBlock * C, nv, width, counts, place, w.k2, [&] { count_ids<false>(r, b, 1, rows, width, lo, counts); });
+                if (chosen.inside && chosen.a >= lo && chosen.a < lo + cap) ya = chosen.y(w, counts.at((int)(chosen.a - lo)));
+            }
+        } else {
+            add_columns<E, RULES>(run, w, x, c0 * cap + place, kBlock * C, (int)(c1 - c0) * nv, width, counts, place, w.k2, [] {});
         }
-        join<kBlock>(run, k2, lds);
+        join<kBlock>(run, w.k2, lds);
         if (threadIdx.x == 0) {
-            if (splits == 1) finish(run, w, the_ya, b, log_prob, entropy, log_sum);
-            else parts[i] = Part{run, the_ya};
+            if (splits == 1) finish(run, w, ya, b, log_prob, entropy, log_sum);
+            else parts[i] = Part{run, ya};
         }
         __syncthreads();
     }
@@ -252,8 +302,9 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
         const int64_t own = band * (kBlock / kWave) + threadIdx.x / kWave;
         const int64_t b = own < rows ? own : rows - 1;
         const Row w = row_of<false>(r, b);
-        Run run{-INFINITY, 0, 0, 0};
+        Run run{-INFINITY, 0, 0};
         if (lane < splits) run = parts[b * splits + lane].run;
+        rebase(run, group_reduce<kWave>(run.m, Max<float>(), (float*)nullptr), w.k2);
         join<kWave>(run, w.k2, nullptr);
         if (lane == 0 && own < rows) {
             const int64_t a = action_of(actions, act64, b);
@@ -262,7 +313,7 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
     }
 }
 
-// Tiles of nv vectors a lane: half as many where the counts take 32 bits.  (Without rules kTile: their loop over vectors is unrolled.)
+// Tiles of nv vectors a lane: half as many where the counts take 32 bits.
 int tile_vectors(const Rules& r) { return r.hist && !half_counts(r) ? kTile / 2 : kTile; }
 
 // As many parts as bring 1024 workgroups, 64 at most, none without a tile.
@@ -305,11 +356,17 @@ struct Launch {
     void* ws;
     hipStream_t s;
 
-    template <int G, int NV, int C>
+    template <int G, int C>
     void in_registers() const {
         constexpr int per = kBlock / G;
-        hipLaunchKernelGGL((score_rows_kernel<E, RULES, G, NV, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r,
-                           (int)((width + G * C - 1) / (G * C)), half_counts(r), actions, act64, lp, ent, ls);
+        hipLaunchKernelGGL((score_rows_kernel<E, RULES, G, C>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r, actions, act64, lp,
+                           ent, ls);
+    }
+    template <int G>
+    void strips(int64_t nv) const {
+        constexpr int per = kBlock / G;
+        hipLaunchKernelGGL((score_strips_kernel<E, RULES, G>), dim3(grid_for((rows + per - 1) / per)), dim3(kBlock), 0, s, x, rows, width, stride, r, (int)nv,
+                           half_counts(r), actions, act64, lp, ent, ls);
     }
     void wide(int nv) const {
         const Split p = split_of(E::kVec, nv, rows, width);
@@ -322,18 +379,27 @@ struct Launch {
     void operator()() const {
         constexpr int v = E::kVec;
         const int most = tile_vectors(r);
-        // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then several vectors
-        if (width <= 2) in_registers<1, 1, 2>();
-        else if (width <= 4) in_registers<1, 1, 4>();
-        else if (width <= v) in_registers<1, 1, v>();
-        else if (width <= 2 * v) in_registers<2, 1, v>();
-        else if (width <= 4 * v) in_registers<4, 1, v>();
-        else if (width <= 8 * v) in_registers<8, 1, v>();
-        else if (width <= 16 * v) in_registers<16, 1, v>();
-        else if (width <= 32 * v) in_registers<32, 1, v>();
-        else if (width <= 64 * v) in_registers<64, 1, v>();
-        else if (width <= 64 * v * most) in_registers<64, kTile, v>();
-        else if (width <= (int64_t)kBlock * v * most) in_registers<kBlock, kTile, v>();
+        const auto need = [&](int g) { return (width + g * v - 1) / (g * v); };   // vectors a lane
+        // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then several vectors: by a wave a row where
+        // there are rows enough (bf16 8192 x 2,083: 14 us, by a workgroup a row 30; f32 4096 x 8,192: 22 and 27; f32 1024 x 8,192: 15 and 10), by a workgroup,
+        // and in parts where few rows are long (f32 64 x 32,768: 12 us, unsplit 20)
+        int g = 1;
+        while (g < kWave && width > g * v) g *= 2;
+        g = lanes_for(r, rows, g);
+        if (width <= kWave * v && g <= kWave) {
+            if (g == 1 && width <= 2) in_registers<1, 2>();
+            else if (g == 1 && width <= 4) in_registers<1, 4>();
+            else if (g == 1) in_registers<1, v>();
+            else if (g == 2) in_registers<2, v>();
+            else if (g == 4) in_registers<4, v>();
+            else if (g == 8) in_registers<8, v>();
+            else if (g == 16) in_registers<16, v>();
+            else if (g == 32) in_registers<32, v>();
+            else in_registers<64, v>();
+        }
+        else if (need(kWave) <= most && g <= kWave) strips<kWave>(need(kWave));
+        else if (!r.hist && need(kWave) <= 32 && rows >= 128 * need(kWave)) strips<kWave>(need(kWave));
+        else if (need(kBlock) <= most || (!r.hist && (need(kBlock) <= 8 || rows >= 1024))) strips<kBlock>(need(kBlock));
         else wide(most);
     }
 };
