@@ -291,6 +291,25 @@ __device__ inline void bias_cols(const Row& w, int64_t v0, int64_t width, float*
     }
 }
 
+// Workgroup i of rows * cuts, cuts to a row.  Adjacent workgroups go to the 8 XCDs in turn, each with an L2 of its own: eight rows are taken side by side, so that
+// a row's cuts, which all read its history, share one; in another order each time, so that dearer rows at a regular distance are spread over the XCDs.
+// (512 x 131,072 bf16 after 4,096 ids, us: process_logits 96 -> 85, sample_actions under all rules 196 -> 177.)
+struct Cut {
+    int64_t row;
+    uint32_t cut;
+    __device__ Cut(int64_t i, uint32_t cuts, int64_t rows) {
+        if (cuts == 1) {
+            row = i;
+            cut = 0;
+            return;
+        }
+        const int64_t eight = i / (8 * cuts);
+        const uint32_t rest = (uint32_t)(i - eight * (8 * cuts)), side = rows - eight * 8 < 8 ? (uint32_t)(rows - eight * 8) : 8u;
+        cut = rest / side;
+        row = eight * 8 + (rest - cut * side + (uint32_t)(eight & 7)) % side;
+    }
+};
+
 // How often ids occur in a tile of columns of n rows, in LDS: 32 bits each, or 16 where no history is longer than 65,535; and with `bits` a bit for
 // each id that occurs at all, behind the counts (cap is a multiple of 32 then).
 struct Counts {
@@ -456,7 +475,7 @@ constexpr int counts_words() { return kBlock * E::kVec * kTile / 2 + kBlock * E:
 inline bool half_counts(const Rules& r) { return r.hist_cols <= 65535; }
 
 // Lanes that share a row which `least` lanes hold: more of them where a history is to be counted and the rows alone do not make the 2,048 workgroups that
-// fill the chip (1,339 rows of 3 columns after 12,191 ids each, 256 lanes instead of one: 3,400 -> NNN us).
+// fill the chip (1,339 rows of 3 columns after 12,191 ids each, 256 lanes instead of one: 3,430 -> 178 us).
 inline int lanes_for(const Rules& r, int64_t rows, int least) {
     int g = least;
     while (g < kBlock && r.hist && r.hist_cols > 4 * g && rows * g < 2048 * kBlock) g *= 2;
