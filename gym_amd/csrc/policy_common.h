@@ -473,6 +473,12 @@ constexpr int kTile = 4;
 template <typename E>
 constexpr int counts_words() { return kBlock * E::kVec * kTile / 2 + kBlock * E::kVec * kTile / 32; }
 inline bool half_counts(const Rules& r) { return r.hist_cols <= 65535; }
+// Where a lane goes through its row vector by vector (sample_actions, action_log_prob) a workgroup's tile under a history is 8,192 columns whatever their type, or 4,096
+// counted in 32 bits: 17 KB.  Of a wave's row it is half as much, for four rows 34 KB: four workgroups a CU, as many as there are registers for.
+template <int G>
+constexpr int strip_words() { return (G == kWave ? 2 : 1) * (8192 / 2 + 8192 / 32); }
+template <typename E>
+int strip_vectors(const Rules& r, int lanes) { return (lanes == kWave ? 2 : 1) * (half_counts(r) ? 8192 : 4096) / (kBlock * E::kVec); }
 
 // Lanes that share a row which `least` lanes hold: more of them where a history is to be counted and the rows alone do not make the 2,048 workgroups that
 // fill the chip (1,339 rows of 3 columns after 12,191 ids each, 256 lanes instead of one: 3,430 -> 178 us).

@@ -377,9 +377,9 @@ template <typename E, bool RULES, int G>
 __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_strips_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys,
                                                                int nv, bool half, int32_t* actions, float* log_prob) {
     constexpr int C = E::kVec, per = kBlock / G;
-    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ __align__(16) uint32_t words[RULES ? strip_words<G>() : 4];
     __shared__ double lds[kBlock / kWave];
-    __shared__ double sums[per][kLong];
+    __shared__ double few[per][RULES ? 8192 / (kWave * E::kVec) : kLong];   // sums of vectors; of many, where there are no counts, in their place
     __shared__ int lds_at;
     const int cap = G * C * nv;
     const int lane = (int)threadIdx.x & (G - 1), group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : 0;
@@ -395,13 +395,14 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_strips_kernel(co
         v.load(w, x, p.at, width);
         if (hist) count_ids(r, band * per, per, rows, width, 0, counts);
         const Heat c = w;
+        double* const sums = RULES && !hist ? (double*)words + group * kLong : few[group];
         long long first = 0;
         bool kept;
-        const Mass mass = sum_strip<E, RULES, G, true>(x, v, w, p, nv, c, lds, &first, sums[group], &kept);
+        const Mass mass = sum_strip<E, RULES, G, true>(x, v, w, p, nv, c, lds, &first, sums, &kept);
         int64_t at = first;
         if (!w.greedy && !mass.bad && mass.base > -INFINITY) {   // the group's lanes alike
-            if (!kept) strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums[group]);
-            at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums[group], &lds_at);
+            if (!kept) strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums);
+            at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums, &lds_at);
         }
         if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob, nullptr);
     }
@@ -418,7 +419,7 @@ template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_parts_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int nv, bool half,
                                                               int64_t cuts, Part* parts) {
     constexpr int C = E::kVec;
-    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ __align__(16) uint32_t words[RULES ? strip_words<kBlock>() : 4];
     __shared__ double lds[kBlock / kWave];
     const int cap = kBlock * C * nv, place = (int)threadIdx.x * C;
     const bool hist = RULES && r.hist;
@@ -443,8 +444,8 @@ template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_join_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, Keys keys, int nv,
                                                              bool half, int64_t cuts, const Part* parts, int32_t* actions, float* log_prob) {
     constexpr int C = E::kVec;
-    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
-    __shared__ double sums[kTile * (kBlock / kWave)];
+    __shared__ __align__(16) uint32_t words[RULES ? strip_words<kBlock>() : 4];
+    __shared__ double sums[8192 / (kWave * E::kVec)];
     __shared__ int lds_at;
     const int cap = kBlock * C * nv, place = (int)threadIdx.x * C, lane = (int)threadIdx.x & (kWave - 1);
     const bool hist = RULES && r.hist;
@@ -499,9 +500,8 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_join_kernel(cons
     }
 }
 
-// Vectors a lane in a strip, at most: what the counts' LDS holds.  (Without a history there could be more; of 8 or 16 the parts take 5 us less of
-// 512 x 131,072 bf16, and the join, which goes through one strip once more, 10 to 15 us more.)
-int strip_vectors(const Rules& r) { return r.hist && !half_counts(r) ? kTile / 2 : kTile; }
+// (Without a history the wide form's strips could be longer; of twice or four times the columns the parts take 5 us less of 512 x 131,072 bf16, and the join,
+// which goes through one strip once more, 10 to 15 us more.)
 int64_t cuts_of(int vec, int nv, int64_t width) {
     const int64_t cap = (int64_t)kBlock * vec * nv;
     return (width + cap - 1) / cap;
@@ -517,7 +517,7 @@ int wide_nv(int vec, int most, int64_t rows, int64_t width) {
 size_t parts_bytes(int64_t rows, int64_t width) {
     size_t most = 0;
     for (const int vec : {F32::kVec, F16::kVec})
-        for (const int nv : {kTile / 2, kTile}) {
+        for (const int nv : {4096 / (kBlock * vec), 8192 / (kBlock * vec)}) {
             const size_t bytes = sizeof(Part) * (size_t)rows * (size_t)cuts_of(vec, wide_nv(vec, nv, rows, width), width);
             if (width > (int64_t)kBlock * vec * nv && bytes > most) most = bytes;
         }
@@ -556,7 +556,7 @@ struct Launch {
     }
     void operator()() const {
         constexpr int v = E::kVec;
-        const int most = strip_vectors(r);
+        const int most = strip_vectors<E>(r, kBlock), wave_most = strip_vectors<E>(r, kWave);
         const auto need = [&](int g) { return (int)((width + g * v - 1) / (g * v)); };   // vectors a lane
         // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then strips
         int g = 1;
@@ -573,8 +573,8 @@ struct Launch {
             else if (g == 32) vectors<32, v>();
             else vectors<64, v>();
         }
-        else if (width <= kWave * v * most && g <= kWave) strips<kWave>(need(kWave));
-        else if (!r.hist && need(kWave) <= kLong && rows >= 128 * need(kWave)) strips<kWave>(need(kWave));
+        else if (need(kWave) <= (r.hist ? wave_most : kLong) && (need(kWave) <= 4 || rows >= 128 * need(kWave)) && (g <= kWave || rows >= 128 * need(kWave)))
+            strips<kWave>(need(kWave));
         else if (need(kBlock) <= most || (!r.hist && need(kBlock) <= kLong / 4 && (need(kBlock) <= 8 || rows >= 16 * need(kBlock)))) strips<kBlock>(need(kBlock));
         else wide(wide_nv(v, most, rows, width));
     }

@@ -229,7 +229,7 @@ template <typename E, bool RULES, int G>
 __global__ void __launch_bounds__(kBlock) score_strips_kernel(const typename E::T* x0, int64_t rows, int64_t width, int64_t stride, Rules r, int nv, bool half,
                                                               const void* actions, int act64, float* log_prob, float* entropy, double* log_sum) {
     constexpr int C = E::kVec, per = kBlock / G;
-    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ __align__(16) uint32_t words[RULES ? strip_words<G>() : 4];
     __shared__ Run lds[kBlock / kWave];
     const int cap = G * C * nv;
     const int lane = (int)threadIdx.x & (G - 1), group = G == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / G) : 0;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) score_wide_kernel(const
                                                             int64_t cuts, int splits, int64_t each, const void* actions, int act64, float* log_prob,
                                                             float* entropy, double* log_sum, Part* parts) {
     constexpr int C = E::kVec;
-    __shared__ __align__(16) uint32_t words[RULES ? counts_words<E>() : 4];
+    __shared__ __align__(16) uint32_t words[RULES ? strip_words<kBlock>() : 4];
     __shared__ Run lds[kBlock / kWave];
     const int cap = kBlock * C * nv, place = (int)threadIdx.x * C;
     const bool hist = RULES && r.hist;
@@ -314,9 +314,6 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
     }
 }
 
-// Tiles of nv vectors a lane: half as many where the counts take 32 bits.
-int tile_vectors(const Rules& r) { return r.hist && !half_counts(r) ? kTile / 2 : kTile; }
-
 // As many parts as bring 1024 workgroups, 64 at most, none without a tile.
 struct Split {
     int64_t cuts, each;
@@ -337,7 +334,7 @@ Split split_of(int vec, int nv, int64_t rows, int64_t width) {
 size_t parts_bytes(int64_t rows, int64_t width) {
     size_t most = 0;
     for (const int vec : {F32::kVec, F16::kVec})
-        for (const int nv : {kTile / 2, kTile}) {
+        for (const int nv : {4096 / (kBlock * vec), 8192 / (kBlock * vec)}) {
             const Split s = split_of(vec, nv, rows, width);
             const size_t bytes = s.splits > 1 ? sizeof(Part) * (size_t)rows * (size_t)s.splits : 0;
             if (width > (int64_t)kBlock * vec * nv && bytes > most) most = bytes;
@@ -379,7 +376,7 @@ struct Launch {
     }
     void operator()() const {
         constexpr int v = E::kVec;
-        const int most = tile_vectors(r);
+        const int most = strip_vectors<E>(r, kBlock), wave_most = strip_vectors<E>(r, kWave);
         const auto need = [&](int g) { return (width + g * v - 1) / (g * v); };   // vectors a lane
         // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then several vectors: by a wave a row where
         // there are rows enough (bf16 8192 x 2,083: 14 us, by a workgroup a row 30; f32 4096 x 8,192: 22 and 27; f32 1024 x 8,192: 15 and 10), by a workgroup,
@@ -398,8 +395,8 @@ struct Launch {
             else if (g == 32) in_registers<32, v>();
             else in_registers<64, v>();
         }
-        else if (need(kWave) <= most && g <= kWave) strips<kWave>(need(kWave));
-        else if (!r.hist && need(kWave) <= 32 && rows >= 128 * need(kWave)) strips<kWave>(need(kWave));
+        else if (need(kWave) <= (r.hist ? wave_most : 32) && (need(kWave) <= 4 || rows >= 128 * need(kWave)) && (g <= kWave || rows >= 128 * need(kWave)))
+            strips<kWave>(need(kWave));
         else if (need(kBlock) <= most || (!r.hist && (need(kBlock) <= 8 || rows >= 1024))) strips<kBlock>(need(kBlock));
         else wide(most);
     }
