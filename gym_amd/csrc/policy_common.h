@@ -577,6 +577,8 @@ __device__ inline double log2_double(double s) {
     const double e = __builtin_fma(a, exp2_double(-l, 1.0), -1.0);
     return __builtin_fma(__builtin_fma(__builtin_fma(e, 1.0 / 3.0, -0.5), e, 1.0) * e, 1.4426950408889634074, l) + (double)n;
 }
+// As a float that is not infinite: a temperature may be so low that its reciprocal overflows, and what is 0 beside it is to stay 0.
+__device__ inline float finite(double v) { return (float)__builtin_fmin(v, 3e38); }
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 

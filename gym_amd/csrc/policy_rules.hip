@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kBlock, RULES ? 5 : 1) score_backward_kernel(c
         const double ls = log_sum[2 * b + 1];
         s.empty = ls == -INFINITY;
         s.ls2 = (float)(ls * kLog2e);
-        s.inv_temp = (float)(1.0 / s.temp);
-        s.k = (float)s.k2;
+        s.inv_temp = finite(1.0 / s.temp);
+        s.k = finite(s.k2);
         s.gl = !g_lp || log_prob[b] == -INFINITY ? 0.f : g_lp[b];
         s.ge = g_ent ? g_ent[b] : 0.f;
         s.ent = entropy[b];

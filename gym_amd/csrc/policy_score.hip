@@ -1,6 +1,6 @@
 // policy_score.hip — log-probability and entropy of given actions under the ruled logits: one pass over the logits with a running maximum.
 //
-// With y the logit after penalties and bias, m a float about the greatest y, t = (y - m) log2 e / T and w = 2^t:  S = sum w, D = sum w t,
+// With y the logit after penalties and bias, m the greatest y so far, t = (y - m) log2 e / T and w = 2^t:  S = sum w, D = sum w t,
 // log_prob = (y_a - m) / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to y - m, not to y); a lane adds up
 // at most 32 of them before it goes on in double.  m is the same for a wave, so that the sums hardly ever have to be brought to a new one: a few times in
 // a row, by the logarithm of its length.  8.5 vector instructions a column, of the 16 that 2-byte logits leave time for at the memory's rate.
@@ -12,14 +12,13 @@ namespace {
 
 // A running (m, S, D) over any set of columns, S and D against m.  A NaN or +inf among them makes S NaN; m = -inf: nothing yet.
 struct Run {
-    float m;
-    double s, d;
+    double m, s, d;
 };
 
 // S and D of r against another base m > r.m.
-__device__ inline void rebase(Run& r, float m, double k2) {
+__device__ inline void rebase(Run& r, double m, double k2) {
     if (r.m > -INFINITY && r.m < m) {
-        double t = ((double)r.m - (double)m) * k2;
+        double t = (r.m - m) * k2;
         t = t > -200 ? t : -200;   // 0 at float32's precision
         const double e = exp2_double(t, 1.0);
         r.d = e * __builtin_fma(t, r.s, r.d);   // against the new base every t moves by the same amount
@@ -34,16 +33,15 @@ __device__ inline void add_term(float t, float& s, float& d) {
     s += w;
     d = __builtin_fmaf(w, __builtin_fmaxf(t, -200.f), d);
 }
-__device__ inline float gap(float y, float m) { return y - m; }
-__device__ inline float gap(double y, float m) { return (float)(y - (double)m); }
 
-// N columns' y of every lane of the wave added to the lanes' runs, whose m is the wave's.
+// N columns' y of every lane of the wave added to the lanes' runs, whose m is the wave's.  Floats are taken from m's nearest float, and what that is off by is
+// added where t is made: m may be the y of a penalty, and the column that holds it has t = 0.
 template <int N, typename Y>
 __device__ inline void add_cols(Run& run, const Y* y, double k2) {
-    float top = (float)y[0];
+    Y top = y[0];
 #pragma unroll
-    for (int j = 1; j < N; j++) top = __builtin_fmaxf(top, (float)y[j]);
-    if (__any(!(top <= run.m))) rebase(run, group_reduce<kWave>(__builtin_fmaxf(top, run.m), Max<float>(), (float*)nullptr), k2);
+    for (int j = 1; j < N; j++) top = __builtin_elementwise_max(top, y[j]);
+    if (__any(!((double)top <= run.m))) rebase(run, group_reduce<kWave>(__builtin_fmax((double)top, run.m), Max<double>(), (double*)nullptr), k2);
     if (run.m == -INFINITY) {
         bool nan = false;
 #pragma unroll
@@ -51,10 +49,11 @@ __device__ inline void add_cols(Run& run, const Y* y, double k2) {
         if (nan) run.s = NAN;
         return;
     }
-    const float k = (float)k2, m = run.m;
+    const float k = finite(k2), m = (float)run.m;
+    const float off = m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * k2);
     float s = 0, d = 0;
 #pragma unroll
-    for (int j = 0; j < N; j++) add_term(gap(y[j], m) * k, s, d);
+    for (int j = 0; j < N; j++) add_term(sizeof(Y) == 4 ? __builtin_fmaf((float)y[j] - m, k, off) : (float)(y[j] - run.m) * k, s, d);
     run.s += (double)s;
     run.d += (double)d;
 }
@@ -114,8 +113,8 @@ __device__ inline void join(Run& run, double k2, Run* lds) {
     __syncthreads();
     if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = run;
     __syncthreads();
-    float m = lds[0].m;
-    for (int i = 1; i < kBlock / kWave; i++) m = __builtin_fmaxf(m, lds[i].m);
+    double m = lds[0].m;
+    for (int i = 1; i < kBlock / kWave; i++) m = __builtin_fmax(m, lds[i].m);
     run = Run{m, 0, 0};
     for (int i = 0; i < kBlock / kWave; i++) {
         Run one = lds[i];
@@ -137,9 +136,9 @@ __device__ inline void finish(const Run& run, const Row& w, double ya, int64_t b
     const double l2 = empty ? 0.0 : log2_double(run.s), ls = l2 * kLn2;
     double inv = empty ? 0.0 : __builtin_amdgcn_rcp(run.s);   // and a Newton step: 1e-14 of it
     inv = __builtin_fma(__builtin_fma(-run.s, inv, 1.0), inv, inv);
-    log_prob[b] = empty ? -INFINITY : (float)(((ya - (double)run.m) * w.k2 - l2) * kLn2);
+    log_prob[b] = empty ? -INFINITY : (float)(((ya - run.m) * w.k2 - l2) * kLn2);
     entropy[b] = empty ? 0.f : (float)((l2 - run.d * inv) * kLn2);
-    log_sum[2 * b] = empty ? 0.0 : (double)run.m;   // apart: beside a mask of the type's lowest value the sum of the two would lose log S
+    log_sum[2 * b] = empty ? 0.0 : run.m;   // apart: beside a mask of the type's lowest value the sum of the two would lose log S
     log_sum[2 * b + 1] = empty ? -INFINITY : ls;
 }
 
@@ -157,21 +156,21 @@ __device__ inline double y_at(const Row& w, const typename E::T* x, int64_t widt
 // The run of a group whose lanes hold all of its columns, C each: the greatest first, the sums against it.
 template <int G, int C, typename Y>
 __device__ inline Run run_of(const Y* y, double k2) {
-    float m = -INFINITY;
+    Y m = -INFINITY;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < C; j++) {
         bad = bad || !(y[j] < (Y)INFINITY);
-        m = __builtin_fmaxf(m, (float)y[j]);
+        m = __builtin_elementwise_max(m, y[j]);
     }
-    m = group_reduce<G>(bad ? (float)INFINITY : m, Max<float>(), (float*)nullptr);
-    if (m == INFINITY) return Run{m, NAN, 0};
-    if (m == -INFINITY) return Run{m, 0, 0};
-    const float k = (float)k2;
+    m = group_reduce<G>(bad ? (Y)INFINITY : m, Max<Y>(), (Y*)nullptr);
+    if (m == (Y)INFINITY) return Run{(double)m, NAN, 0};
+    if (m == -(Y)INFINITY) return Run{(double)m, 0, 0};
+    const float k = finite(k2);
     float s = 0, d = 0;
 #pragma unroll
-    for (int j = 0; j < C; j++) add_term(gap(y[j], m) * k, s, d);
-    return Run{m, (double)group_reduce<G>(s, Sum<float>(), (float*)nullptr), (double)group_reduce<G>(d, Sum<float>(), (float*)nullptr)};
+    for (int j = 0; j < C; j++) add_term((float)(y[j] - m) * k, s, d);
+    return Run{(double)m, (double)group_reduce<G>(s, Sum<float>(), (float*)nullptr), (double)group_reduce<G>(d, Sum<float>(), (float*)nullptr)};
 }
 
 // The action of a row and its logit, read early: both are on their way while the row is summed.
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(kBlock) score_join_kernel(int64_t rows, int64_
         const Row w = row_of<false>(r, b);
         Run run{-INFINITY, 0, 0};
         if (lane < splits) run = parts[b * splits + lane].run;
-        rebase(run, group_reduce<kWave>(run.m, Max<float>(), (float*)nullptr), w.k2);
+        rebase(run, group_reduce<kWave>(run.m, Max<double>(), (double*)nullptr), w.k2);
         join<kWave>(run, w.k2, nullptr);
         if (lane == 0 && own < rows) {
             const int64_t a = action_of(actions, act64, b);
