@@ -35,13 +35,18 @@ __device__ inline void add_term(float t, float& s, float& d) {
 }
 
 // N columns' y of every lane of the wave added to the lanes' runs, whose m is the wave's.  Floats are taken from m's nearest float, and what that is off by is
-// added where t is made: m may be the y of a penalty, and the column that holds it has t = 0.
-template <int N, typename Y>
+// added where t is made: m may be the y of a penalty, and the column that holds it has t = 0.  LOGITS: no y is anything but a logit, m is a float.
+template <int N, bool LOGITS, typename Y>
 __device__ inline void add_cols(Run& run, const Y* y, double k2) {
     Y top = y[0];
 #pragma unroll
     for (int j = 1; j < N; j++) top = __builtin_elementwise_max(top, y[j]);
-    if (__any(!((double)top <= run.m))) rebase(run, group_reduce<kWave>(__builtin_fmax((double)top, run.m), Max<double>(), (double*)nullptr), k2);
+    if constexpr (LOGITS) {
+        const float m = (float)run.m;
+        if (__any(!(top <= m))) rebase(run, (double)group_reduce<kWave>(__builtin_fmaxf(top, m), Max<float>(), (float*)nullptr), k2);
+    } else {
+        if (__any(!((double)top <= run.m))) rebase(run, group_reduce<kWave>(__builtin_fmax((double)top, run.m), Max<double>(), (double*)nullptr), k2);
+    }
     if (run.m == -INFINITY) {
         bool nan = false;
 #pragma unroll
@@ -50,7 +55,7 @@ __device__ inline void add_cols(Run& run, const Y* y, double k2) {
         return;
     }
     const float k = finite(k2), m = (float)run.m;
-    const float off = m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * k2);
+    const float off = LOGITS || m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * k2);
     float s = 0, d = 0;
 #pragma unroll
     for (int j = 0; j < N; j++) add_term(sizeof(Y) == 4 ? __builtin_fmaf((float)y[j] - m, k, off) : (float)(y[j] - run.m) * k, s, d);
@@ -86,19 +91,19 @@ __device__ inline void add_columns(Run& run, const Row& w, const typename E::T* 
 #pragma unroll
                 for (int j = 0; j < C; j++) y[j] = v.bits >> j & 1 ? y[j] : -INFINITY;
             }
-            add_cols<C>(run, y, k2);
+            add_cols<C, false>(run, y, k2);
         } else {
             float y[C];
 #pragma unroll
             for (int j = 0; j < C; j++) y[j] = v.raw.get(j);
-            add_cols<C>(run, y, k2);
+            add_cols<C, !RULES>(run, y, k2);
         }
         if constexpr (RULES) {
             while (__any(apart)) {   // lanes without one add nothing
                 const int j = __ffs((int)apart) - 1;
                 const double y = apart ? ruled(w, whole.pick(j < 0 ? 0 : j), counts.at(place + k * step + (j < 0 ? 0 : j)), true, at + j) : -(double)INFINITY;
                 apart &= apart - 1;
-                add_cols<1>(run, &y, k2);
+                add_cols<1, false>(run, &y, k2);
             }
         }
     }
