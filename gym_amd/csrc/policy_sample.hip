@@ -19,8 +19,6 @@ struct Place {
     int64_t at, width;
     int step, place;
     Counts counts;   // words null: no history
-
-    __device__ bool inside(int k) const { return at + k * step < width; }
 };
 
 // f(y) for the y of vector k: floats where they are the logits themselves, else (under a bias, or where a lane of the wave has a count) doubles.
@@ -558,7 +556,8 @@ struct Launch {
         constexpr int v = E::kVec;
         const int most = strip_vectors<E>(r, kBlock), wave_most = strip_vectors<E>(r, kWave);
         const auto need = [&](int g) { return (int)((width + g * v - 1) / (g * v)); };   // vectors a lane
-        // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then strips
+        // few columns: a row per lane, as wide as the row; then as few lanes as hold it, a 16-byte vector each; then strips (kLong has the figures), of a wave
+        // where they are short or there are rows enough, of a workgroup up to 8 vectors a lane or where there are rows enough, else parts
         int g = 1;
         while (g < kWave && width > g * v) g *= 2;
         g = lanes_for(r, rows, g);

@@ -151,13 +151,6 @@ __device__ inline int64_t action_of(const void* actions, int act64, int64_t b) {
     return act64 ? ((const int64_t*)actions)[b] : (int64_t)((const int32_t*)actions)[b];
 }
 
-// y of one column, -inf outside the row or where it is not allowed.
-template <typename E>
-__device__ inline double y_at(const Row& w, const typename E::T* x, int64_t width, int64_t v, uint32_t count) {
-    if (v < 0 || v >= width) return -INFINITY;
-    return ruled(w, (float)x[v], count, allowed(w, v), v);
-}
-
 // The run of a group whose lanes hold all of its columns, C each: the greatest first, the sums against it.
 template <int G, int C, typename Y>
 __device__ inline Run run_of(const Y* y, double k2) {
