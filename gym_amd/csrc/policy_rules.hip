@@ -19,11 +19,17 @@ template <typename E>
 Tiling tiling(int64_t rows, int64_t width, const Rules& r) {
     Tiling t;
     t.half = half_counts(r);
+    const int64_t most = r.hist && !t.half ? kTile / 2 : kTile;
+    // As few lanes as hold a row in `most` vectors each, for what a row costs beside its columns is paid by each of its waves; more where rows are too few for 2,048
+    // workgroups, or a lane would have more than 80 ids to count.  us against a vector a lane: 18,315 x 1,086 f16 after 10 ids 82 -> 37, 1,000,000 x 18 f32 with a
+    // bias 76 -> 40, none 41 -> 36; after 300 ids 410 -> 360 (462 without the rule for ids, 430 and 1,130 for 9 bf16 columns).
     t.lanes_log2 = 0;
-    while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) < width) t.lanes_log2++;
+    while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) * (width <= E::kVec ? 1 : most) < width) t.lanes_log2++;
+    while (t.lanes_log2 < 8 && ((int64_t)E::kVec << t.lanes_log2) < width && (rows << t.lanes_log2 < 2048 * kBlock || (r.hist && r.hist_cols > 80u << t.lanes_log2)))
+        t.lanes_log2++;
     for (const int lanes = lanes_for(r, rows, 1 << t.lanes_log2); 1 << t.lanes_log2 < lanes;) t.lanes_log2++;
     const int64_t step = (int64_t)E::kVec << t.lanes_log2;
-    const int64_t need = (width + step - 1) / step, most = r.hist && !t.half ? kTile / 2 : kTile;
+    const int64_t need = (width + step - 1) / step;
     t.nv = (int)(need < most ? need : most);
     t.cuts = (width + step * t.nv - 1) / (step * t.nv);
     const int64_t per = kBlock >> t.lanes_log2;
