@@ -188,16 +188,16 @@ __device__ inline int walk(const double* e, double s, double before, double leve
     return (first & (W - 1)) * C + at;
 }
 
-// A row's answer, by one lane: `at` its chosen column unless there is none, and that column's weight.  The logarithm of a weight by itself and the sum's
+// A row's answer, by one lane: `at` its chosen column unless there is none, and where the lane has them that column's weight and logit.  The logarithm of a weight by itself and the sum's
 // differ by 1e-16 of y: a column that is all of the sum has probability 1 for certain, and none has more.
 template <typename E>
 __device__ inline void answer(const Row& w, const typename E::T* x, const Mass& mass, int64_t at, uint32_t count, const Heat& c, int64_t b,
-                              int32_t* actions, float* log_prob, const double* chosen) {
+                              int32_t* actions, float* log_prob, const double* chosen, const float* logit) {
     const bool none = mass.bad || mass.base == -INFINITY;
     actions[b] = none ? -1 : (int32_t)at;
     float lp = mass.bad ? NAN : -INFINITY;
     if (!none) {
-        const double y = ruled(w, (float)x[at], count, true, at) - mass.base;
+        const double y = ruled(w, logit ? *logit : (float)x[at], count, true, at) - mass.base;
         const double share = chosen ? *chosen : weight(y, c);
         lp = share >= mass.sum ? 0.0f : (float)__builtin_fmin((y * c.k2 - log2_double(mass.sum)) * kLn2, 0.0);
     }
@@ -243,10 +243,14 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_vectors_kernel(c
         int64_t at = walk<G, C>(e, s, 0.0, row_uniform(keys, b) * mass.sum, mass.sum * 0x1p-80);
         if (w.greedy) at = first;
         double chosen = e[0];
+        float logit = v.raw.get(0);
 #pragma unroll
-        for (int j = 1; j < C; j++) chosen = at == j ? e[j] : chosen;
+        for (int j = 1; j < C; j++) {
+            chosen = at == j ? e[j] : chosen;
+            logit = at == j ? v.raw.get(j) : logit;
+        }
         if (lane == 0 && own < rows)
-            answer<E>(w, x, mass, at, hist && at < width ? words[group * cap + at] : 0u, c, b, actions, log_prob, G == 1 ? &chosen : nullptr);
+            answer<E>(w, x, mass, at, hist && at < width ? words[group * cap + at] : 0u, c, b, actions, log_prob, G == 1 ? &chosen : nullptr, G == 1 ? &logit : nullptr);
     }
 }
 
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_strips_kernel(co
             if (!kept) strip_sums<E, RULES, G>(x, v, w, p, nv, c, mass.base, sums);
             at = locate<E, RULES, G>(x, w, p, nv, c, mass.base, mass.sum, row_uniform(keys, b) * mass.sum, sums, &lds_at);
         }
-        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob, nullptr);
+        if (lane == 0 && own < rows) answer<E>(w, x, mass, at, hist && at < width ? counts.at(group * cap + (int)at) : 0u, c, b, actions, log_prob, nullptr, nullptr);
     }
 }
 
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_join_kernel(cons
             strip_sums<E, RULES, kBlock>(x, v, w, p, nv, scale, base, sums);
             at = lo + locate<E, RULES, kBlock>(x, w, p, nv, scale, base, parts_b[c].sum, target, sums, &lds_at);
         }
-        if (threadIdx.x == 0) answer<E>(w, x, mass, at, any && hist ? counts.at((int)(at % cap)) : 0u, scale, b, actions, log_prob, nullptr);
+        if (threadIdx.x == 0) answer<E>(w, x, mass, at, any && hist ? counts.at((int)(at % cap)) : 0u, scale, b, actions, log_prob, nullptr, nullptr);
         __syncthreads();
     }
 }
