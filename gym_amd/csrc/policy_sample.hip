@@ -10,7 +10,8 @@ namespace gymhip {
 namespace policy {
 namespace {
 
-// A weight: 2^(d k2), d = y - base.
+// A weight: 2^(d k2), d = y - base; never 0, for it stops at 2^-1000: what cannot be chosen (a masked column, one behind the row's end) weighs that much, and walk and
+// find_part tell it by its size.
 __device__ inline double weight(double d, const Heat& c) { return exp2_double(__builtin_fmax(d, c.least), c.k2); }
 
 // Where a lane stands in its row: `at` its first column, `step` the columns from one of its vectors to the next, `place` its first column's place in
@@ -49,8 +50,10 @@ __device__ inline double weigh(const Y* y, double base, const Heat& c, double* e
     return s;
 }
 // The same against 0.  A double holds 2^-900 .. 2^900 at full precision, so nothing has to be known of the greatest y beforehand: this is all there
-// is to do where no y is above `most` nor a NaN and the row's sum is not below 2^-900.  *beyond: the wave's lanes that have such a y (as a lane mask: one
+// is to do where no y is above `most` nor a NaN and the row's sum is above kLeastSum.  The level is 2^-53 of that at least, beside which a double does not see the weights
+// of 2^-1000: in one lane's running sum they are nothing.  *beyond: the wave's lanes that have such a y (as a lane mask: one
 // vector instruction a column).
+constexpr double kLeastSum = 0x1p-800;
 template <int C, typename Y>
 __device__ inline double weigh_0(const Y* y, const Heat& c, double* e, uint64_t* beyond) {
     double s = 0;
@@ -158,8 +161,10 @@ __device__ inline Mass sum_against_max(const typename E::T* x, const Row& w, con
     return mass;
 }
 
-// The column (0 = the first of the lanes' vectors) of W lanes' vectors that the running sum passes `level` in: e[] a lane's weights, s their sum.
-// Should rounding leave the level above all sums, the last column with any weight is taken; weights up to `tiny` count as none to that.
+// The column (0 = the first of the lanes' vectors) of W lanes' vectors that the running sum passes `level` in: e[] a lane's weights, s their sum.  The lanes' running sums are
+// added up in different orders, so one may pass the level by a last bit in a lane, or a column, that adds nothing.  Hence what weighs at most `tiny`, 2^-80 of the whole, is
+// not chosen: columns up to `tiny`, and lanes up to twice C of those (a lane with more has a column with more, whatever its sum's rounding).
+// Should rounding leave the level above all sums, the last column that counts is taken.
 template <int W, int C>
 __device__ inline int walk(const double* e, double s, double before, double level, double tiny) {
     const int self = (int)(threadIdx.x & (kWave - 1)), lane = self & (W - 1);
@@ -167,7 +172,7 @@ __device__ inline int walk(const double* e, double s, double before, double leve
     int first = self;
     if (W > 1) {
         const uint64_t group = W == 64 ? ~0ull : ((1ull << W) - 1) << (self & ~(W - 1));
-        const uint64_t hits = __ballot(s > 0 && before + upto > level) & group, any = __ballot(s > tiny) & group;
+        const uint64_t any = __ballot(s > tiny * (2 * C)) & group, hits = __ballot(before + upto > level) & any;
         first = hits ? __ffsll((unsigned long long)hits) - 1 : any ? 63 - __clzll((long long)any) : self;
     }
     // every lane walks its own vector; the chosen lane's answer counts
@@ -176,7 +181,7 @@ __device__ inline int walk(const double* e, double s, double before, double leve
 #pragma unroll
     for (int j = 0; j < C; j++) {
         acc += e[j];
-        at = at == C && acc > level ? j : at;
+        at = at == C && acc > level && (W == 1 || e[j] > tiny) ? j : at;   // (a lane by itself adds in the columns' order, see kLeastSum)
     }
     if (__any(at == C)) {
         int last = 0;
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_vectors_kernel(c
         uint64_t beyond = 0;
         with_y<E, RULES, C>(w, p, 0, v, [&](const auto* y) { s = weigh_0<C>(y, c, e, &beyond); });
         Mass mass{0.0, group_reduce<G>(w.greedy || mine_in(beyond) ? (double)NAN : s, Sum<double>(), (double*)nullptr), false};
-        const bool whole = mass.sum > 0x1p-900;
+        const bool whole = mass.sum > kLeastSum;
         long long first = 0;
         if (__any(!whole)) {   // the same for all lanes that exchange
             const Mass other = sum_against_max<E, RULES, G, C>(x, w, p, 1, c, nullptr, &first);
@@ -254,8 +259,8 @@ __global__ void __launch_bounds__(kBlock, RULES ? 4 : 1) sample_vectors_kernel(c
     }
 }
 
-// Where the running sum of n parts passes `level`, 64 parts at a time, by each wave for itself: the part, or the last one with more than `tiny` should
-// rounding leave the level above all sums (*past); *before: what comes before it.
+// Where the running sum of n parts passes `level`, 64 parts at a time, by each wave for itself: the part, or the last one should rounding leave the level
+// above all sums (*past); *before: what comes before it.  Parts of at most `tiny` are not chosen (see walk).
 template <typename F>
 __device__ inline int64_t find_part(int64_t n, double level, double tiny, F part_sum, double* before, bool* past) {
     const int lane = (int)threadIdx.x & (kWave - 1);
@@ -264,7 +269,7 @@ __device__ inline int64_t find_part(int64_t n, double level, double tiny, F part
     for (int64_t c0 = 0; c0 < n; c0 += kWave) {
         const double e = c0 + lane < n ? part_sum(c0 + lane) : 0.0;
         const double upto = running_sum<kWave>(e, lane);
-        const uint64_t hits = __ballot(e > 0 && run + upto > level), some = __ballot(e > tiny);
+        const uint64_t some = __ballot(e > tiny), hits = __ballot(run + upto > level) & some;
         if (hits) {
             const int at = __ffsll((unsigned long long)hits) - 1;
             *before = run + __shfl(upto - e, at);
@@ -336,7 +341,7 @@ __device__ inline Mass sum_strip(const typename E::T* x, const Vector<E, E::kVec
             each_vector<E>(w, x, p, nv, v0, [&](int k, const Vector<E, C>& v) { sum += weigh_apart<E, RULES>(w, p, k, v, c, &beyond); });
             sum = group_reduce<G>(mine_in(beyond) ? (double)NAN : sum, Sum<double>(), lds);
         }
-        if (sum > 0x1p-900) {
+        if (sum > kLeastSum) {
             if (KEEP) *kept = true;
             return Mass{0.0, sum, false};
         }
@@ -354,7 +359,8 @@ __device__ inline int locate(const typename E::T* x, const Row& w, const Place& 
     const double tiny = sum * 0x1p-80;
     double before;
     bool past;
-    const int part = __builtin_amdgcn_readfirstlane((int)find_part(nv * M, level, tiny, [&](int64_t i) { return sums[i]; }, &before, &past));   // (vector, wave)
+    // (a wave's 64 vectors with more than this have a lane with more than walk's 2 C tiny; one of at most 256 such parts has)
+    const int part = __builtin_amdgcn_readfirstlane((int)find_part(nv * M, level, tiny * (256 * C), [&](int64_t i) { return sums[i]; }, &before, &past));   // (vector, wave)
     if (past) level = INFINITY;
     const int k = part / M, at_wave = part - k * M;
     int column = 0;
