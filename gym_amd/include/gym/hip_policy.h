@@ -70,6 +70,8 @@ inline at::Tensor side(const at::Tensor& t, const char* what, const at::Device& 
 
 inline int intType(const at::Tensor& t) { return t.scalar_type() == at::kLong ? GYMHIP_ACT_I64 : GYMHIP_ACT_I32; }
 inline void* stream(const at::Tensor& x) { return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream(); }
+// t is written through its pointer, which autograd does not see: whoever has saved it (or a view of it) has to find it changed.  Inference tensors cannot be saved.
+inline void written(const at::Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 inline at::Tensor emptyLike(const at::Tensor& x) { return at::empty(x.sizes(), x.options()); }
 
 }  // namespace detail
@@ -326,16 +328,20 @@ inline at::Tensor processLogits(const at::Tensor& logits, const LogitRules* rule
     detail::process(x, *b, out);
     return out;
 }
-// The same into `out`, which may be the logits themselves, or memory that does not touch them; not under autograd.
+// The same into `out`, which may be the logits themselves, or memory that does not touch them; not under autograd.  A change of `out` in place, for
+// whoever has saved it for a backward pass.
 inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules, at::Tensor out) {
     const at::Tensor x = detail::ready(logits, "logits");
     detail::require(!at::GradMode::is_enabled() || !(logits.requires_grad() || out.requires_grad()), "out= is not available under autograd");
     detail::require(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device() &&
                     (out.stride(1) == 1 || out.size(1) <= 1), "out must have the logits' shape, type and device, and adjacent columns");
-    detail::process(x, *detail::bind(rules, x), out);
+    const detail::BoundPtr b = detail::bind(rules, x);
+    detail::written(out);
+    detail::process(x, *b, out);
 }
 
-// One action per row from softmax(z) (int32; -1 where nothing can be chosen) and its log-probability (float32, no gradient).
+// One action per row from softmax(z) (int32; -1 where nothing can be chosen) and its log-probability (float32, no gradient).  Into `actions` and `log_prob`
+// where they are given, which is a change of them in place.
 inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits, const LogitRules* rules, const Keys& keys, at::Tensor actions = {},
                                                         at::Tensor log_prob = {}) {
     const at::Tensor x = detail::ready(logits, "logits");
@@ -352,6 +358,8 @@ inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits
     const detail::BoundKeys k(keys, n, x.device());
     const size_t bytes = gymhip_sample_workspace_bytes(n, width);
     const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : at::Tensor();
+    detail::written(actions);
+    detail::written(log_prob);
     const c10::OptionalDeviceGuard guard(x.device());
     detail::check(gymhip_sample_actions(x.data_ptr(), detail::typeOf(x.scalar_type()), n, width, x.stride(0), b->ptr(), &k.c, actions.data_ptr<int32_t>(),
                                         log_prob.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, detail::stream(x)), "gymhip_sample_actions");

@@ -87,7 +87,7 @@ def _rules(rules):
 
 def process_logits(logits: torch.Tensor, rules: LogitRules | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """z (LogitRules) of logits [rows, width], rounded once to their type.  Differentiable in the logits.  `out` (not under autograd) may
-    be the logits themselves, or memory that does not touch them."""
+    be the logits themselves, or memory that does not touch them.  It changes in place: a backward pass that has saved it raises."""
     if out is None:
         return _ext.process_logits(logits, _rules(rules))
     _ext.process_logits_into(logits, _rules(rules), out)
@@ -100,7 +100,9 @@ def sample_actions(logits: torch.Tensor, rules: LogitRules | None = None, *, see
     has rows + b) or int64 [rows]; `step` is a number, an int64 device scalar (one for all rows, read when the kernel runs: advance it
     between replays of a captured graph) or int64 [rows].  Keys and steps count modulo 2^48.
 
-    A row with nothing allowed gives action -1 and log-probability -inf, a row with a NaN or +inf among its allowed z -1 and NaN."""
+    A row with nothing allowed gives action -1 and log-probability -inf, a row with a NaN or +inf among its allowed z -1 and NaN.
+
+    `out`'s tensors change in place: a backward pass that has saved them (action_log_prob saves its actions) raises."""
     if out is None:
         return ActionSample(*_ext.sample_actions(logits, _rules(rules), seed, step, rows))
     _ext.sample_actions(logits, _rules(rules), seed, step, rows, *out)
