@@ -341,9 +341,10 @@ inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules,
 }
 
 // One action per row from softmax(z) (int32; -1 where nothing can be chosen) and its log-probability (float32, no gradient).  Into `actions` and `log_prob`
-// where they are given, which is a change of them in place.
+// where both are given, which is a change of them in place.
 inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits, const LogitRules* rules, const Keys& keys, at::Tensor actions = {},
                                                         at::Tensor log_prob = {}) {
+    detail::require(actions.defined() == log_prob.defined(), "out needs both actions and log_prob, or neither");
     const at::Tensor x = detail::ready(logits, "logits");
     const int64_t n = x.size(0), width = x.size(1);
     if (actions.defined()) {
