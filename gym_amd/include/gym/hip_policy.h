@@ -44,23 +44,31 @@ inline at::Tensor rowwise(const at::Tensor& x) {
     return (x.stride(1) == 1 || x.size(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous();
 }
 
-inline at::Tensor ready(const at::Tensor& x, const char* what) {
+// Forward-mode derivatives are not made, and what carries a tangent has no requires_grad to tell: refused, where its tangent would be lost.
+inline void noTangent(const at::Tensor& x, const char* what) {
+    if (x._fw_grad(0).defined()) throw std::runtime_error(std::string(what) + " carries a forward-mode derivative, which the policy operators do not have");
+}
+
+// derived: the result has a derivative in x.
+inline at::Tensor ready(const at::Tensor& x, const char* what, bool derived = true) {
     require(x.dim() == 2, std::string(what) + " must be a 2-D tensor [rows, width]");
     require(typeOf(x.scalar_type()) >= 0, std::string(what) + " must be float32, float16 or bfloat16, got " + at::toString(x.scalar_type()));
+    if (derived) noTangent(x, what);
     if (!x.is_cuda()) throw Error(std::string(what) + " is on " + x.device().str() + ": the policy kernels run on the GPU and have no CPU fallback");
     require(x.size(1) <= GYMHIP_POLICY_MAX_WIDTH, std::string(what) + ": at most 2^24 columns, got " + std::to_string(x.size(1)));
     return rowwise(x);
 }
 
-// A tensor beside the logits: its type, device and shape checked; adjacent along its last axis.
+// A tensor beside the logits: its type, device and shape checked; adjacent along its last axis.  derived: the result has derivatives, if none in t.
 inline at::Tensor side(const at::Tensor& t, const char* what, const at::Device& device, std::initializer_list<at::ScalarType> types,
-                       std::initializer_list<std::vector<int64_t>> shapes) {
+                       std::initializer_list<std::vector<int64_t>> shapes, bool derived = true) {
     bool ok = false;
     std::string names;
     for (auto s : types) { ok = ok || t.scalar_type() == s; names += (names.empty() ? "" : " or ") + std::string(at::toString(s)); }
     require(ok, std::string(what) + " must be a tensor of " + names);
     require(t.device() == device, std::string(what) + " is on " + t.device().str() + ", the logits on " + device.str());
     require(!t.requires_grad(), std::string(what) + " requires a gradient: only the logits have one");
+    if (derived) noTangent(t, what);
     ok = false;
     names.clear();
     for (auto const& s : shapes) { ok = ok || t.sizes() == at::IntArrayRef(s); names += (names.empty() ? "" : " or ") + shapeOf(s); }
@@ -124,7 +132,7 @@ struct Bound : torch::CustomClassHolder {
     const gymhip_logit_rules* ptr() const { return any ? &c : nullptr; }
 
     Bound() = default;
-    Bound(const LogitRules& r, const at::Tensor& logits) : any(true) {
+    Bound(const LogitRules& r, const at::Tensor& logits, bool derived = true) : any(true) {
         r.check();
         const int64_t rows = logits.size(0), width = logits.size(1), words = (width + 31) / 32;
         const at::Device dev = logits.device();
@@ -142,7 +150,7 @@ struct Bound : torch::CustomClassHolder {
             if (r.mask_rows.defined()) c.mask_rows = (const int32_t*)held(side(r.mask_rows, "mask_rows", dev, {at::kInt}, {{rows}}));
         }
         if (r.bias.defined()) {
-            at::Tensor b = side(r.bias, "bias", dev, {at::kFloat}, {{width}, {1, width}, {rows, width}});
+            at::Tensor b = side(r.bias, "bias", dev, {at::kFloat}, {{width}, {1, width}, {rows, width}}, derived);
             if (b.dim() == 2 && b.stride(0) < 0) b = b.contiguous();
             c.bias = (const float*)held(b);
             c.bias_stride = b.dim() == 2 && b.size(0) > 1 ? b.stride(0) : 0;
@@ -164,10 +172,10 @@ struct Bound : torch::CustomClassHolder {
                 }
             }
         }
-        value(r.repetition, "repetition", rows, dev, &c.repetition, &c.repetition_rows);
-        value(r.presence, "presence", rows, dev, &c.presence, &c.presence_rows);
-        value(r.frequency, "frequency", rows, dev, &c.frequency, &c.frequency_rows);
-        value(r.temperature, "temperature", rows, dev, &c.temperature, &c.temperature_rows);
+        value(r.repetition, "repetition", rows, dev, derived, &c.repetition, &c.repetition_rows);
+        value(r.presence, "presence", rows, dev, derived, &c.presence, &c.presence_rows);
+        value(r.frequency, "frequency", rows, dev, derived, &c.frequency, &c.frequency_rows);
+        value(r.temperature, "temperature", rows, dev, derived, &c.temperature, &c.temperature_rows);
     }
 
 private:
@@ -175,14 +183,14 @@ private:
         keep.push_back(t);
         return t.data_ptr();
     }
-    void value(const PerRow& v, const char* name, int64_t rows, const at::Device& dev, float* number, const float** per_row) {
-        if (v.rows.defined()) *per_row = (const float*)held(side(v.rows, name, dev, {at::kFloat}, {{rows}}));
+    void value(const PerRow& v, const char* name, int64_t rows, const at::Device& dev, bool derived, float* number, const float** per_row) {
+        if (v.rows.defined()) *per_row = (const float*)held(side(v.rows, name, dev, {at::kFloat}, {{rows}}, derived));
         else *number = (float)v.number;
     }
 };
 using BoundPtr = c10::intrusive_ptr<Bound>;
-inline BoundPtr bind(const LogitRules* rules, const at::Tensor& logits) {
-    return rules ? c10::make_intrusive<Bound>(*rules, logits) : c10::make_intrusive<Bound>();
+inline BoundPtr bind(const LogitRules* rules, const at::Tensor& logits, bool derived = true) {
+    return rules ? c10::make_intrusive<Bound>(*rules, logits, derived) : c10::make_intrusive<Bound>();
 }
 
 }  // namespace detail
@@ -331,6 +339,7 @@ inline at::Tensor processLogits(const at::Tensor& logits, const LogitRules* rule
 // The same into `out`, which may be the logits themselves, or memory that does not touch them; not under autograd.  A change of `out` in place, for
 // whoever has saved it for a backward pass.
 inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules, at::Tensor out) {
+    detail::noTangent(out, "out");
     const at::Tensor x = detail::ready(logits, "logits");
     detail::require(!at::GradMode::is_enabled() || !(logits.requires_grad() || out.requires_grad()), "out= is not available under autograd");
     detail::require(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device() &&
@@ -345,7 +354,7 @@ inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules,
 inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits, const LogitRules* rules, const Keys& keys, at::Tensor actions = {},
                                                         at::Tensor log_prob = {}) {
     detail::require(actions.defined() == log_prob.defined(), "out needs both actions and log_prob, or neither");
-    const at::Tensor x = detail::ready(logits, "logits");
+    const at::Tensor x = detail::ready(logits, "logits", false);
     const int64_t n = x.size(0), width = x.size(1);
     if (actions.defined()) {
         detail::side(actions, "out.actions", x.device(), {at::kInt}, {{n}});
@@ -355,7 +364,7 @@ inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits
         actions = at::empty({n}, x.options().dtype(at::kInt));
         log_prob = at::empty({n}, x.options().dtype(at::kFloat));
     }
-    const detail::BoundPtr b = detail::bind(rules, x);
+    const detail::BoundPtr b = detail::bind(rules, x, false);
     const detail::BoundKeys k(keys, n, x.device());
     const size_t bytes = gymhip_sample_workspace_bytes(n, width);
     const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : at::Tensor();

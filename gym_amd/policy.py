@@ -16,7 +16,8 @@ gym_amd.vec_env calls them from VecLogitActions (step(logits)) and VecObservatio
 
 
 The tensors' checks, the autograd nodes and the calls of the C ABI are C++ (include/gym/hip_policy.h, which C++ trainers include themselves), bound in
-csrc/policy_torch.cpp.  Wrong values raise ValueError, wrong Python types TypeError, and what fails or finds no GPU GymhipError.
+csrc/policy_torch.cpp.  Wrong values raise ValueError, wrong Python types TypeError, and what fails or finds no GPU GymhipError.  There are first derivatives in
+reverse mode: a second one (create_graph) and tensors with a forward-mode tangent raise RuntimeError.
 """
 from __future__ import annotations
 
