@@ -35,7 +35,8 @@ __device__ inline void add_term(float t, float& s, float& d) {
 }
 
 // N columns' y of every lane of the wave added to the lanes' runs, whose m is the wave's.  Floats are taken from m's nearest float, and what that is off by is
-// added where t is made: m may be the y of a penalty, and the column that holds it has t = 0.  LOGITS: no y is anything but a logit, m is a float.
+// added where t is made: m may be the y of a penalty, and the column that holds it has t = 0.  Both by the same factor: a temperature's reciprocal that passes float32 is
+// cut off (`finite`), and if the one were and the other not, t could rise above 0.  LOGITS: no y is anything but a logit, m is a float.
 template <int N, bool LOGITS, typename Y>
 __device__ inline void add_cols(Run& run, const Y* y, double k2) {
     Y top = y[0];
@@ -55,7 +56,7 @@ __device__ inline void add_cols(Run& run, const Y* y, double k2) {
         return;
     }
     const float k = finite(k2), m = (float)run.m;
-    const float off = LOGITS || m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * k2);
+    const float off = LOGITS || m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * __builtin_fmin(k2, 3e38));
     float s = 0, d = 0;
 #pragma unroll
     for (int j = 0; j < N; j++) add_term(sizeof(Y) == 4 ? __builtin_fmaf((float)y[j] - m, k, off) : (float)(y[j] - run.m) * k, s, d);
