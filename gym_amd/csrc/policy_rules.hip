@@ -322,6 +322,7 @@ int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules*
     out->heat = Heat::of(1.f);
     if (!r) return GYMHIP_OK;
     if (r->struct_size != (int32_t)sizeof(gymhip_logit_rules)) return fail(GYMHIP_EINVAL, "bad gymhip_logit_rules.struct_size");
+    if (!rows || !width) return GYMHIP_OK;   // there is nothing to rule, and the pointers to a row's things may be null without meaning that there are none
     if (r->mask) {
         if (r->mask_lines < 1) return fail(GYMHIP_EINVAL, "mask_lines must be positive");
         if (!r->mask_rows && r->mask_lines != 1 && r->mask_lines != rows) return fail(GYMHIP_EINVAL, "without mask_rows, mask_lines must be 1 or rows");

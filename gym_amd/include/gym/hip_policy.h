@@ -141,7 +141,7 @@ struct Bound : torch::CustomClassHolder {
             require(r.mask.dim() == 2 && r.mask.size(1) >= words, "mask must be an int32 tensor [lines, >= " + std::to_string(words) + "] for " + std::to_string(width) + " columns");
             require(r.mask_rows.defined() || r.mask.size(0) == 1 || r.mask.size(0) == rows,
                     "mask has " + std::to_string(r.mask.size(0)) + " lines for " + std::to_string(rows) + " rows: one, one per row, or mask_rows");
-            require(r.mask.size(0) > 0, "mask has no lines");
+            require(r.mask.size(0) > 0 || rows == 0, "mask has no lines");
             at::Tensor m = side(r.mask, "mask", dev, {at::kInt}, {r.mask.sizes().vec()});
             if (m.size(0) > 1 && m.stride(0) < words) m = m.contiguous();   // lines that share storage (an expanded mask)
             c.mask = (const uint32_t*)held(m);
@@ -176,6 +176,7 @@ struct Bound : torch::CustomClassHolder {
         value(r.presence, "presence", rows, dev, derived, &c.presence, &c.presence_rows);
         value(r.frequency, "frequency", rows, dev, derived, &c.frequency, &c.frequency_rows);
         value(r.temperature, "temperature", rows, dev, derived, &c.temperature, &c.temperature_rows);
+        any = rows > 0 && width > 0;   // of an empty batch the tensors are checked and no more: their pointers are null, which stands for no rule
     }
 
 private:

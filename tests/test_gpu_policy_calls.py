@@ -114,3 +114,21 @@ def test_temperatures_near_zero_under_a_history(width, temperature, kind):
     assert torch.isfinite(lp).all() and torch.isfinite(ent).all() and torch.isfinite(got).all()
     assert torch.equal(s.actions[sure].cpu().long(), best.cpu()[sure]) and (s.log_prob[sure] == 0).all()
     assert (lp[sure] == 0).all() and (ent[sure] == 0).all() and (got[sure] == 0).all()
+
+
+# ---- empty batches -------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n, width", [(0, 5), (3, 0), (0, 0)])
+@pytest.mark.parametrize("lines", [None, 1, 5])
+def test_nothing_to_do_under_every_rule(n, width, lines):
+    from gym_amd.policy import action_log_prob, process_logits, sample_actions
+    from tests.test_policy_calls import per_row_rules
+    rules = per_row_rules(n, width, "cuda", lines)
+    x = torch.zeros(n, width, device="cuda", requires_grad=True)
+    z = process_logits(x, rules)
+    assert z.shape == (n, width) and torch.autograd.grad(z.sum(), x)[0].shape == (n, width)
+    s = sample_actions(x, rules, seed=1, rows=torch.arange(n).cuda(), step=torch.zeros(n, dtype=torch.int64).cuda())
+    assert s.actions.tolist() == [-1] * n and s.log_prob.tolist() == [-math.inf] * n
+    lp, ent = action_log_prob(x, torch.zeros(n, dtype=torch.int32, device="cuda"), rules)
+    assert lp.tolist() == [-math.inf] * n and ent.tolist() == [0.0] * n
+    assert torch.autograd.grad(ent.sum(), x)[0].shape == (n, width)

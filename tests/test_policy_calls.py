@@ -33,3 +33,46 @@ def test_forward_mode_derivatives_are_refused():
                 rules._bind(x)
         with pytest.raises(L.GymhipError, match="no CPU fallback"):   # not refused for its tangent
             policy.sample_actions(dual, seed=1)
+
+
+# ---- empty batches ---------------------------------------------------------------------------------------------------------------------------
+
+def per_row_rules(n, width, device="cpu", lines=None):
+    """Every tensor that a rule may have, for n rows; with `lines` a table of masks, else a line a row."""
+    words = (width + 31) // 32
+    many = dict(history=torch.zeros(n, 3, dtype=torch.int64, device=device), history_len=torch.zeros(n, dtype=torch.int32, device=device), bias=torch.zeros(n, width, device=device))
+    for name in ("repetition", "presence", "frequency", "temperature"):
+        many[name] = torch.ones(n, device=device)
+    many["mask"] = torch.zeros(n if lines is None else lines, words, dtype=torch.int32, device=device)
+    if lines is not None:
+        many["mask_rows"] = torch.zeros(n, dtype=torch.int32, device=device)
+    return policy.LogitRules(**many)
+
+
+@pytest.mark.parametrize("n, width", [(0, 40), (0, 0), (3, 0)])
+@pytest.mark.parametrize("lines", [None, 1, 5])
+def test_rules_of_an_empty_batch(n, width, lines):
+    per_row_rules(n, width, lines=lines)._bind(torch.zeros(n, width))
+
+
+def test_rules_of_an_empty_batch_are_checked_all_the_same():
+    x = torch.zeros(0, 40)
+    for bad in (dict(mask=torch.zeros(0, 1, dtype=torch.int32)), dict(bias=torch.zeros(0, 39)), dict(history=torch.zeros(2, 3, dtype=torch.int32)),
+                dict(temperature=torch.ones(1)), dict(mask=torch.zeros(5, 2, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            policy.LogitRules(**bad)._bind(x)
+
+
+def test_abi_no_rows_is_no_work_whatever_the_rules_point_to():
+    """The arrays of an empty batch may be null: no pointer of theirs stands for 'none'."""
+    lib, k = L.load(), keys_struct()
+    for rules in (rules_struct(mask=HERE, mask_lines=0, mask_stride=2), rules_struct(mask=HERE, mask_lines=5, mask_stride=2), rules_struct(mask_rows=HERE),
+                  rules_struct(repetition=0.0), rules_struct(history_len=HERE)):
+        r = C.byref(rules)
+        assert process(rows=0, ptr=None, out=None, rules=rules) == 0
+        assert process(rows=2, width=0, stride=0, ptr=None, out=None, out_stride=0, rules=rules) == 0
+        assert lib.gymhip_process_logits_backward(None, L.TYPE_F32, 0, 8, 8, r, None, 8, None, 8, None) == 0
+        assert lib.gymhip_sample_actions(None, L.TYPE_F32, 0, 8, 8, r, C.byref(k), None, None, None, 0, None) == 0
+        assert lib.gymhip_action_log_prob(None, L.TYPE_F32, 0, 8, 8, r, None, L.ACT_I32, None, None, None, None, 0, None) == 0
+        assert lib.gymhip_action_log_prob_backward(None, L.TYPE_F32, 0, 8, 8, r, None, L.ACT_I32, None, None, None, None, None, None, 8, None) == 0
+    refused(process(rows=0, ptr=None, out=None, rules=rules_struct(struct_size=3)), "struct_size")
