@@ -59,7 +59,8 @@ inline at::Tensor ready(const at::Tensor& x, const char* what, bool derived = tr
     return rowwise(x);
 }
 
-// A tensor beside the logits: its type, device and shape checked; adjacent along its last axis.  derived: the result has derivatives, if none in t.
+// A tensor beside the logits: its type, device and shape checked; adjacent along its last axis.  derived: the result has derivatives, but
+// not in t, whose own would be lost.
 inline at::Tensor side(const at::Tensor& t, const char* what, const at::Device& device, std::initializer_list<at::ScalarType> types,
                        std::initializer_list<std::vector<int64_t>> shapes, bool derived = true) {
     bool ok = false;
@@ -67,8 +68,10 @@ inline at::Tensor side(const at::Tensor& t, const char* what, const at::Device& 
     for (auto s : types) { ok = ok || t.scalar_type() == s; names += (names.empty() ? "" : " or ") + std::string(at::toString(s)); }
     require(ok, std::string(what) + " must be a tensor of " + names);
     require(t.device() == device, std::string(what) + " is on " + t.device().str() + ", the logits on " + device.str());
-    require(!t.requires_grad(), std::string(what) + " requires a gradient: only the logits have one");
-    if (derived) noTangent(t, what);
+    if (derived) {
+        require(!(t.requires_grad() && at::GradMode::is_enabled()), std::string(what) + " requires a gradient: only the logits have one");
+        noTangent(t, what);
+    }
     ok = false;
     names.clear();
     for (auto const& s : shapes) { ok = ok || t.sizes() == at::IntArrayRef(s); names += (names.empty() ? "" : " or ") + shapeOf(s); }

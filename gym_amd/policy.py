@@ -65,7 +65,8 @@ class LogitRules(_ext.LogitRules):
     repetition, presence, frequency, temperature   a number, or float32 [rows].  repetition > 0, temperature >= 0; the penalties act through
                   `history` alone.  Temperature 0 leaves z undivided, and sample_actions then takes the greatest z (lowest v of equal ones).
 
-    The tensors are read when an operator runs, not copied here; values of the tensors are not checked."""
+    The tensors are read when an operator runs, not copied here; values of the tensors are not checked.  They have no gradient: under autograd
+    one that requires it is refused by the differentiable operators (sample_actions takes it)."""
 
     __slots__ = ()
 

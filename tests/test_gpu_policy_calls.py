@@ -132,3 +132,23 @@ def test_nothing_to_do_under_every_rule(n, width, lines):
     lp, ent = action_log_prob(x, torch.zeros(n, dtype=torch.int32, device="cuda"), rules)
     assert lp.tolist() == [-math.inf] * n and ent.tolist() == [0.0] * n
     assert torch.autograd.grad(ent.sum(), x)[0].shape == (n, width)
+
+
+# ---- rules that are learned ----------------------------------------------------------------------------------------------------------------------
+
+def test_learned_rules_are_taken_where_no_gradient_is_lost():
+    from gym_amd.policy import ActionSample, LogitRules, action_log_prob, process_logits, sample_actions
+    x, g = logits_of(4, 30, torch.float32, 3)
+    bias, hot = torch.randn(30, generator=g).cuda().requires_grad_(), torch.full((4,), 0.7).cuda().requires_grad_()
+    learned, fixed = LogitRules(bias=bias, temperature=hot), LogitRules(bias=bias.detach(), temperature=hot.detach())
+    a = torch.arange(4).cuda()
+    want = sample_actions(x, fixed, seed=1)
+    got = sample_actions(x, learned, seed=1)   # a draw has no gradient, under autograd or not
+    assert torch.equal(got.actions, want.actions) and torch.equal(got.log_prob, want.log_prob) and not got.log_prob.requires_grad
+    with torch.no_grad():
+        assert torch.equal(process_logits(x, learned), process_logits(x, fixed))
+        assert torch.equal(action_log_prob(x, a, learned)[0], action_log_prob(x, a, fixed)[0])
+    for call in (lambda: process_logits(x, learned), lambda: action_log_prob(x, a, learned), lambda: process_logits(x.clone().requires_grad_(), learned),
+                 lambda: sample_actions(x, seed=1, out=ActionSample(want.actions, want.log_prob.clone().requires_grad_()))):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()

@@ -76,3 +76,17 @@ def test_abi_no_rows_is_no_work_whatever_the_rules_point_to():
         assert lib.gymhip_action_log_prob(None, L.TYPE_F32, 0, 8, 8, r, None, L.ACT_I32, None, None, None, None, 0, None) == 0
         assert lib.gymhip_action_log_prob_backward(None, L.TYPE_F32, 0, 8, 8, r, None, L.ACT_I32, None, None, None, None, None, None, 8, None) == 0
     refused(process(rows=0, ptr=None, out=None, rules=rules_struct(struct_size=3)), "struct_size")
+
+
+# ---- tensors that require a gradient ---------------------------------------------------------------------------------------------------------
+
+def test_rules_that_are_learned():
+    """Refused where their gradient would be lost, taken where there is none to lose."""
+    x = torch.zeros(3, 40)
+    rules = policy.LogitRules(bias=torch.zeros(40, requires_grad=True), temperature=torch.ones(3, requires_grad=True))
+    with pytest.raises(ValueError, match="requires a gradient"):
+        rules._bind(x)
+    with torch.no_grad():
+        rules._bind(x)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        policy.LogitRules(bias=rules.bias)._bind(x)
