@@ -353,10 +353,17 @@ class VecEnvWrapper(VecEnv):
         return self.venv.seed(_seed)
 
 
-def _env_offset(venv):
-    """The global index of the first env under any wrappers: the random-number key of row 0."""
+def _env_offset(venv, told=None):
+    """The global index of the first env under any wrappers, the random-number key of row 0: as told, else what the VecEnv says of itself.  One that says
+    nothing has all envs if it is the only process; of several ranks each would draw the same, so there it must be told."""
+    if told is not None:
+        return int(told)
     while not hasattr(venv, "env_offset") and hasattr(venv, "venv"):
         venv = venv.venv
+    if not hasattr(venv, "env_offset"):
+        import torch.distributed as dist
+        if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+            raise ValueError(f"{type(venv).__name__} has no env_offset: with {dist.get_world_size()} ranks pass env_offset=, the global index of this rank's first env")
     return int(getattr(venv, "env_offset", 0))
 
 
@@ -396,14 +403,15 @@ class VecLogitActions(VecEnvWrapper):
     The draw of env i at step t follows from (seed, i's GLOBAL index, t) alone: neither the GPU count nor the order of the calls matters.
     seed(s) gives the envs their seeds and the draws a new one, and restarts t.  `sample` holds the last step's actions and log-probabilities
     (new tensors each step); action_log_prob scores them again, with gradients.  An env whose rules leave nothing to choose gets action -1.
-    device_step=True keeps t on the GPU, for steps recorded into a graph."""
+    device_step=True keeps t on the GPU, for steps recorded into a graph.  env_offset: the global index of env 0, for a VecEnv that has no such
+    attribute (needed with more than one rank)."""
 
-    def __init__(self, venv: VecEnv, rules=None, seed: int = 0, device_step: bool = False):
+    def __init__(self, venv: VecEnv, rules=None, seed: int = 0, device_step: bool = False, env_offset: int | None = None):
         super().__init__(venv)
         if not isinstance(venv.actionSpace(), spaces.Discrete):
             raise TypeError(f"VecLogitActions needs a Discrete action space, got {venv.actionSpace()!r}")
-        self.rules, self.sample = rules, None
-        self._seed, self._step, self._offset = int(seed), _Counter(device_step), _env_offset(venv)
+        self.rules, self.sample, self.env_offset = rules, None, _env_offset(venv, env_offset)
+        self._seed, self._step = int(seed), _Counter(device_step)
 
     def seed(self, _seed):
         self._seed = int(_seed)
@@ -415,7 +423,7 @@ class VecLogitActions(VecEnvWrapper):
         shape = (self.numEnvs, self.actionSpace().n)
         if tuple(logits.shape) != shape:
             raise ValueError(f"logits have shape {tuple(logits.shape)}, expected {shape}")
-        self.sample = policy.sample_actions(logits, self.rules, seed=self._seed, step=self._step.on(logits.device), rows=self._offset)
+        self.sample = policy.sample_actions(logits, self.rules, seed=self._seed, step=self._step.on(logits.device), rows=self.env_offset)
         self._step.advance()
         self.venv.stepAsync(self.sample.actions)
 
@@ -426,15 +434,15 @@ class VecObservationDropout(VecEnvWrapper):
 
     What is dropped for env i in the t-th observation since seed(s) follows from (seed, i's GLOBAL index, t) alone.  reset(index) has masks
     of its own and leaves t as it is.  training = False passes the observations on untouched (t goes on all the same).
-    device_step=True keeps t on the GPU, for steps recorded into a graph."""
+    device_step=True keeps t on the GPU, for steps recorded into a graph.  env_offset as for VecLogitActions."""
 
-    def __init__(self, venv: VecEnv, p: float, seed: int = 0, device_step: bool = False):
+    def __init__(self, venv: VecEnv, p: float, seed: int = 0, device_step: bool = False, env_offset: int | None = None):
         super().__init__(venv)
         p = float(p)
         if not 0.0 <= p < 1.0 or round(65536 * p) > 65535:
             raise ValueError(f"p must lie in [0, 1) and round to less than 65536 / 65536, got {p}")
-        self.p, self.training = p, True
-        self._seed, self._step, self._offset = int(seed), _Counter(device_step), _env_offset(venv)
+        self.p, self.training, self.env_offset = p, True, _env_offset(venv, env_offset)
+        self._seed, self._step = int(seed), _Counter(device_step)
 
     def seed(self, _seed):
         self._seed = int(_seed)
@@ -449,7 +457,7 @@ class VecObservationDropout(VecEnvWrapper):
     def _next(self, obs):
         step = self._step.on(obs.device)
         if self.training:
-            obs = self._drop(obs, self._offset, step)
+            obs = self._drop(obs, self.env_offset, step)
         self._step.advance()
         return obs
 
@@ -458,7 +466,7 @@ class VecObservationDropout(VecEnvWrapper):
             return self._next(self.venv.reset())
         obs = self.venv.reset(index)
         # the number of the next observation, in the upper half of the steps' 48 bits, which the count does not reach
-        return self._drop(obs.unsqueeze(0), self._offset + int(index), self._step.on(obs.device) + (1 << 47)).squeeze(0) if self.training else obs
+        return self._drop(obs.unsqueeze(0), self.env_offset + int(index), self._step.on(obs.device) + (1 << 47)).squeeze(0) if self.training else obs
 
     def stepWait(self):
         r = self.venv.stepWait()

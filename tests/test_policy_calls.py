@@ -90,3 +90,38 @@ def test_rules_that_are_learned():
         rules._bind(x)
     with pytest.raises(ValueError, match="requires a gradient"):
         policy.LogitRules(bias=rules.bias)._bind(x)
+
+
+# ---- where a wrapper's rows stand among all envs -------------------------------------------------------------------------------------------------
+
+def test_wrappers_take_or_ask_for_the_env_offset(recorded, monkeypatch):
+    """Ranks around envs of unknown offset would all draw the same: the offset is to be told then."""
+    import torch.distributed as dist
+    from gym_amd.vec_env import VecEnvWrapper, VecLogitActions, VecObservationDropout
+
+    def unknown():
+        venv = fake_venv()
+        del type(venv).env_offset
+        return VecEnvWrapper(venv)
+
+    def key(make):
+        del recorded[:]
+        venv = make()
+        venv.reset()
+        if isinstance(venv, VecLogitActions):
+            venv.step(torch.zeros(4, 2))
+        return recorded[-1][3]
+
+    assert key(lambda: VecLogitActions(unknown())) == 0 and key(lambda: VecObservationDropout(unknown(), 0.5)) == 0   # one process has all envs
+    assert key(lambda: VecLogitActions(unknown(), env_offset=33)) == 33 and key(lambda: VecObservationDropout(unknown(), 0.5, env_offset=34)) == 34
+    assert key(lambda: VecLogitActions(fake_venv(), env_offset=0)) == 0   # what is told wins
+    # a wrapper that was told tells those around it
+    assert key(lambda: VecLogitActions(VecObservationDropout(unknown(), 0.5, env_offset=34))) == 34
+    monkeypatch.setattr(dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(dist, "get_world_size", lambda *a: 2)
+    for make in (VecLogitActions, lambda v: VecObservationDropout(v, 0.5)):
+        with pytest.raises(ValueError, match="env_offset"):
+            make(unknown())
+    assert key(lambda: VecLogitActions(unknown(), env_offset=0)) == 0 and key(lambda: VecLogitActions(fake_venv())) == 10
+    monkeypatch.setattr(dist, "get_world_size", lambda *a: 1)
+    assert key(lambda: VecLogitActions(unknown())) == 0
