@@ -304,7 +304,8 @@ int check_matrix(const char* what, const void* data, int type, int64_t rows, int
     return GYMHIP_OK;
 }
 
-// An output's rows must not share elements, and it may coincide with an input only element for element.
+// An output's rows must not share elements, and it may coincide with an input only element for element.  Rows equally far apart may lie between each other (the halves
+// of a buffer's rows); of other layouts the whole ranges must be apart.
 int check_output(const char* what, const void* out, int type, int64_t rows, int64_t width, int64_t stride, const void* in, int64_t in_stride) {
     if (int rc = check_matrix(what, out, type, rows, width, stride)) return rc;
     if (rows > 1 && stride < width) return fail(GYMHIP_EINVAL, "%s: rows overlap (stride < width)", what);
@@ -312,8 +313,12 @@ int check_output(const char* what, const void* out, int type, int64_t rows, int6
     const uintptr_t e = (uintptr_t)element_size(type);
     const uintptr_t a = (uintptr_t)out, a1 = a + ((uintptr_t)(rows - 1) * (uintptr_t)stride + (uintptr_t)width) * e;
     const uintptr_t c = (uintptr_t)in, c1 = c + ((uintptr_t)(rows - 1) * (uintptr_t)in_stride + (uintptr_t)width) * e;
-    if (a < c1 && c < a1) return fail(GYMHIP_EINVAL, "%s overlaps an input", what);
-    return GYMHIP_OK;
+    if (a >= c1 || c >= a1) return GYMHIP_OK;
+    if (rows > 1 && in_stride == stride) {   // from a row of the input to the output's next one, and on to the input's next
+        const uintptr_t s = (uintptr_t)stride * e, w = (uintptr_t)width * e, d = a >= c ? (a - c) % s : (s - (c - a) % s) % s;
+        if (d >= w && s - d >= w) return GYMHIP_OK;
+    }
+    return fail(GYMHIP_EINVAL, "%s overlaps an input", what);
 }
 
 int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules* out) {

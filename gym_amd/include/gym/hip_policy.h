@@ -340,7 +340,7 @@ inline at::Tensor processLogits(const at::Tensor& logits, const LogitRules* rule
     detail::process(x, *b, out);
     return out;
 }
-// The same into `out`, which may be the logits themselves, or memory that does not touch them; not under autograd.  A change of `out` in place, for
+// The same into `out`, which may be the logits themselves, or memory that shares no element with them or the rules' tensors (other columns of the same buffer, say); not under autograd.  A change of `out` in place, for
 // whoever has saved it for a backward pass.
 inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules, at::Tensor out) {
     detail::noTangent(out, "out");

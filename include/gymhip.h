@@ -396,7 +396,8 @@ typedef struct gymhip_random_keys {
 } gymhip_random_keys;
 
 /* z of `logits` [rows][width] (type, element stride between rows) rounded once to the same type.  `out` may be `logits` itself (same
- * stride); any other overlap is GYMHIP_EINVAL. */
+ * stride) or lie between its rows (same stride, no element in common); any other overlap of the two is GYMHIP_EINVAL.  What the rules point to must
+ * not be written by the call. */
 int gymhip_process_logits(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules, void* out,
                           int64_t out_stride, void* stream);
 /* d(logits) from d(z): 0 where the mask's bit is 0. */

@@ -152,3 +152,26 @@ def test_learned_rules_are_taken_where_no_gradient_is_lost():
                  lambda: sample_actions(x, seed=1, out=ActionSample(want.actions, want.log_prob.clone().requires_grad_()))):
         with pytest.raises(ValueError, match="requires a gradient"):
             call()
+
+
+# ---- outputs that lie between the rows of an input -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("width", [1, 5, 64, 1000, 9001])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_logits_and_results_in_one_buffer(dtype, width):
+    """[logits | results] as the two halves of each of a buffer's rows, in either order: they share no element."""
+    from gym_amd.policy import process_logits
+    n = 5
+    x, g = logits_of(n, width, dtype, width)
+    rules = rules_of("all", n, width, g)
+    want = process_logits(x, rules)
+    for first, second in ((0, width), (width, 0), (0, width + 3), (width + 3, 1)):
+        both = torch.full((n, 2 * width + 5), 7.0, dtype=dtype, device="cuda")
+        both[:, first:first + width] = x
+        out = both[:, second:second + width]
+        process_logits(both[:, first:first + width], rules, out=out)
+        assert torch.equal(out, want) and torch.equal(both[:, first:first + width], x)
+        rest = torch.ones(2 * width + 5, dtype=torch.bool, device="cuda")
+        rest[first:first + width] = False
+        rest[second:second + width] = False
+        assert (both[:, rest] == 7).all()

@@ -125,3 +125,10 @@ def test_wrappers_take_or_ask_for_the_env_offset(recorded, monkeypatch):
     assert key(lambda: VecLogitActions(unknown(), env_offset=0)) == 0 and key(lambda: VecLogitActions(fake_venv())) == 10
     monkeypatch.setattr(dist, "get_world_size", lambda *a: 1)
     assert key(lambda: VecLogitActions(unknown())) == 0
+
+
+# ---- outputs that lie between the rows of an input ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows, width, stride, at", [(3, 8, 16, 7), (3, 8, 16, -7), (3, 8, 15, 8), (3, 8, 16, 9), (3, 8, 16, 16), (3, 8, 16, 1), (3, 8, 8, 8), (3, 8, 16, 39), (1, 8, 0, 7), (1, 8, 16, -7)])
+def test_outputs_that_share_elements_with_an_input_are_refused(rows, width, stride, at):
+    refused(process(rows=rows, width=width, stride=stride, out_stride=stride, out=HERE + 4 * at), "overlaps an input")
