@@ -180,7 +180,7 @@ struct Heat {
     static __host__ __device__ Heat of(float t) {
         Heat h;
         h.greedy = !(t > 0.f);
-        h.temp = h.greedy ? 1.0 : t < 3e38f ? (double)t : 3e38;
+        h.temp = h.greedy ? 1.0 : t < INFINITY ? (double)t : 3.4028234663852886e38;   // an infinite one (values of tensors are not checked): as the greatest float
         h.k2 = 1.4426950408889634074 / h.temp;
         const double unit = h.temp * 0.69314718055994530942, most = 900.0 * unit;
         h.least = -1000.0 * unit;

@@ -13,6 +13,8 @@
 #include <torch/torch.h>
 
 #include <cmath>
+#include <limits>
+#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -120,8 +122,12 @@ struct LogitRules {
 private:
     static void number(const PerRow& v, const char* name, bool positive, bool not_negative) {
         if (v.rows.defined()) return;
-        detail::require(std::abs(v.number) < 3e38 && (!positive || v.number > 0) && (!not_negative || v.number >= 0),
-                        std::string(name) + " must be finite" + (positive ? ", and positive" : not_negative ? ", and not negative" : "") + "; got " + std::to_string(v.number));
+        // as the kernels take it: a number too small for float32 must not turn into the 0 that stands for something else
+        const bool fits = std::abs(v.number) <= std::numeric_limits<float>::max(), positive_f = (float)v.number > 0;
+        std::ostringstream got;
+        got << v.number;
+        detail::require(fits && (!positive || positive_f) && (!not_negative || positive_f || v.number == 0),
+                        std::string(name) + " must be a finite float32" + (positive ? ", and positive" : not_negative ? ", and not negative" : "") + "; got " + got.str());
     }
 };
 

@@ -132,3 +132,15 @@ def test_wrappers_take_or_ask_for_the_env_offset(recorded, monkeypatch):
 @pytest.mark.parametrize("rows, width, stride, at", [(3, 8, 16, 7), (3, 8, 16, -7), (3, 8, 15, 8), (3, 8, 16, 9), (3, 8, 16, 16), (3, 8, 16, 1), (3, 8, 8, 8), (3, 8, 16, 39), (1, 8, 0, 7), (1, 8, 16, -7)])
 def test_outputs_that_share_elements_with_an_input_are_refused(rows, width, stride, at):
     refused(process(rows=rows, width=width, stride=stride, out_stride=stride, out=HERE + 4 * at), "overlaps an input")
+
+
+# ---- numbers at the ends of float32 ----------------------------------------------------------------------------------------------------------------
+
+def test_numbers_that_float32_does_not_hold():
+    for kw in (dict(temperature=1e-50), dict(temperature=7e-46), dict(temperature=1e39), dict(repetition=1e-50), dict(repetition=1e39), dict(presence=-1e39), dict(frequency=1e39)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            policy.LogitRules(**kw)
+    top = torch.finfo(torch.float32).max
+    policy.LogitRules(temperature=top, repetition=top, presence=-top, frequency=top)._bind(torch.zeros(3, 40))
+    policy.LogitRules(temperature=1e-45, repetition=1e-45, presence=1e-50, frequency=-1e-50)._bind(torch.zeros(3, 40))
+    policy.LogitRules(temperature=0.0)._bind(torch.zeros(3, 40))
