@@ -5,6 +5,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/gymhip.h"
@@ -589,6 +590,12 @@ int check_rules(const gymhip_logit_rules* r, int64_t rows, int64_t width, Rules*
 int check_keys(const gymhip_random_keys* k, Keys* out);
 int check_actions(const void* actions, int dtype, int64_t rows);
 int check_workspace(const void* workspace, size_t bytes, size_t needed);
+struct Range {
+    const char* what;
+    const void* at;
+    int64_t bytes;
+};
+int check_results(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, std::initializer_list<Range> results);
 int launched();
 
 // Workgroups for n units of work: as many as there are, up to `most`; kernels stride over the rest.

@@ -379,6 +379,19 @@ int check_workspace(const void* workspace, size_t bytes, size_t needed) {
     return GYMHIP_OK;
 }
 
+// What is written per row must lie in none of the logits, of which other rows are still read then, nor in another result.
+int check_results(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, std::initializer_list<Range> results) {
+    if (!rows) return GYMHIP_OK;
+    const Range x{"logits", logits, width ? ((rows - 1) * stride + width) * element_size(type) : 0};
+    const auto cross = [](const Range& a, const Range& b) { return (uintptr_t)a.at < (uintptr_t)b.at + (uintptr_t)b.bytes && (uintptr_t)b.at < (uintptr_t)a.at + (uintptr_t)a.bytes; };
+    for (const Range* r = results.begin(); r != results.end(); r++) {
+        if (cross(*r, x)) return fail(GYMHIP_EINVAL, "%s overlaps the logits", r->what);
+        for (const Range* q = results.begin(); q != r; q++)
+            if (cross(*r, *q)) return fail(GYMHIP_EINVAL, "%s overlaps %s", r->what, q->what);
+    }
+    return GYMHIP_OK;
+}
+
 int launched() {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GYMHIP_OK : fail(GYMHIP_EHIP, "launch failed: %s", hipGetErrorString(e));

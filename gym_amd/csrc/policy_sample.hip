@@ -612,6 +612,7 @@ int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t wi
     if (int rc = check_keys(keys, &k)) return rc;
     if (rows && (!actions || !log_prob)) return fail(GYMHIP_EINVAL, "actions or log_prob is null");
     if (int rc = check_workspace(workspace, workspace_bytes, gymhip_sample_workspace_bytes(rows, width))) return rc;
+    if (int rc = check_results(logits, type, rows, width, stride, {{"actions", actions, rows * 4}, {"log_prob", log_prob, rows * 4}})) return rc;
     if (!rows) return GYMHIP_OK;
     return with_type(type, [&](auto e) {
         using E = decltype(e);

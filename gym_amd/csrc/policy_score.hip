@@ -423,6 +423,7 @@ int gymhip_action_log_prob(const void* logits, int type, int64_t rows, int64_t w
     if (int rc = check_actions(actions, action_dtype, rows)) return rc;
     if (rows && (!log_prob || !entropy || !log_sum)) return fail(GYMHIP_EINVAL, "log_prob, entropy or log_sum is null");
     if (int rc = check_workspace(workspace, workspace_bytes, gymhip_action_log_prob_workspace_bytes(rows, width))) return rc;
+    if (int rc = check_results(logits, type, rows, width, stride, {{"log_prob", log_prob, rows * 4}, {"entropy", entropy, rows * 4}, {"log_sum", log_sum, rows * 16}})) return rc;
     if (!rows) return GYMHIP_OK;
     return with_type(type, [&](auto e) {
         using E = decltype(e);

@@ -105,7 +105,7 @@ def sample_actions(logits: torch.Tensor, rules: LogitRules | None = None, *, see
 
     A row with nothing allowed gives action -1 and log-probability -inf, a row with a NaN or +inf among its allowed z -1 and NaN.
 
-    `out`'s tensors change in place: a backward pass that has saved them (action_log_prob saves its actions) raises."""
+    `out`'s tensors must lie neither in the logits nor in each other.  They change in place: a backward pass that has saved them (action_log_prob saves its actions) raises."""
     if out is None:
         return ActionSample(*_ext.sample_actions(logits, _rules(rules), seed, step, rows))
     _ext.sample_actions(logits, _rules(rules), seed, step, rows, *out)

@@ -353,7 +353,7 @@ int gymhip_host_env_post_step(int64_t n, const float* reward_in, const uint8_t* 
  * The policy's end of the VecEnv loop: logits to actions, their scores with gradients, dropout.  NO COUNTERPART IN THE REFERENCE
  * (its trainer is outside the repository; VecEnv::step takes finished actions, base.h:56-63).  Stateless: every pointer is device
  * memory of the CURRENT device, calls enqueue on `stream`, allocate nothing and may be recorded into a HIP graph; two calls at once
- * need two workspaces.  rows = 0 is allowed and does nothing, width = 0 is rows that allow nothing; either way the rules' pointers are not looked at.
+ * need two workspaces.  Results of a row each must lie neither in the logits nor in each other (GYMHIP_EINVAL).  rows = 0 is allowed and does nothing, width = 0 is rows that allow nothing; either way the rules' pointers are not looked at.
  * ==================================================================================================================== */
 enum { GYMHIP_TYPE_F32 = 0, GYMHIP_TYPE_F16 = 1, GYMHIP_TYPE_BF16 = 2 };
 /* The widest row of logits or features.  Offsets are 64-bit: rows x stride is not limited. */

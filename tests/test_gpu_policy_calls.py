@@ -295,3 +295,19 @@ def test_dropout_of_more_blocks_than_one_trip(n, width, dtype, trip):
         keep = R.kept(cut.stop - cut.start, width, 0.25, 3, rows=9 + cut.start)
         want = torch.where(keep, x[cut].cpu().double() * (4 / 3), 0.0)
         assert ((y[cut].cpu().double() - want).abs() <= (half_step(dtype) + 2 * U) * want.abs()).all()
+
+
+# ---- results that lie in what is still read ------------------------------------------------------------------------------------------------------
+
+def test_drawn_results_in_the_logits_or_in_each_other_are_refused():
+    from gym_amd._lib import GymhipError
+    from gym_amd.policy import ActionSample, sample_actions
+    x, _ = logits_of(6, 1, torch.float32, 1)
+    store = torch.zeros(40, device="cuda")
+    actions = torch.zeros(6, dtype=torch.int32, device="cuda")
+    for a, lp in ((actions, x[:, 0]), (x[:, 0].view(torch.int32), store[:6]), (store[:6].view(torch.int32), store[5:11])):
+        with pytest.raises(GymhipError, match="overlaps"):
+            sample_actions(x, seed=1, out=ActionSample(a, lp))
+    # side by side in one buffer is apart
+    got = sample_actions(x, seed=1, out=ActionSample(store[:6].view(torch.int32), store[6:12]))
+    assert got.actions.tolist() == [0] * 6 and got.log_prob.tolist() == [0.0] * 6 and (store[12:] == 0).all()

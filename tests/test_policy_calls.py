@@ -144,3 +144,19 @@ def test_numbers_that_float32_does_not_hold():
     policy.LogitRules(temperature=top, repetition=top, presence=-top, frequency=top)._bind(torch.zeros(3, 40))
     policy.LogitRules(temperature=1e-45, repetition=1e-45, presence=1e-50, frequency=-1e-50)._bind(torch.zeros(3, 40))
     policy.LogitRules(temperature=0.0)._bind(torch.zeros(3, 40))
+
+
+# ---- results that lie in what is still read --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("actions, log_prob, text", [(8, 4096, "actions overlaps"), (4096, 40, "log_prob overlaps"), (4096, 4096, "log_prob overlaps"), (4096, 4100, "log_prob overlaps"),
+                                                     (-4, 4096, "actions overlaps")])
+def test_drawn_results_in_the_logits_or_in_each_other_are_refused(actions, log_prob, text):
+    """Other rows are read after a row's answer is written.  Two rows of 8 float32, 12 apart: 80 bytes of logits."""
+    k = keys_struct()
+    refused(L.load().gymhip_sample_actions(HERE, L.TYPE_F32, 2, 8, 12, None, C.byref(k), HERE + actions, HERE + log_prob, None, 0, None), text)
+
+
+@pytest.mark.parametrize("log_prob, entropy, log_sum, text", [(72, 4096, 8192, "log_prob overlaps"), (4096, 0, 8192, "entropy overlaps"), (4096, 8192, 64, "log_sum overlaps"),
+                                                              (4096, 4100, 8192, "entropy overlaps"), (4096, 8192, 8184, "log_sum overlaps")])
+def test_scores_in_the_logits_or_in_each_other_are_refused(log_prob, entropy, log_sum, text):
+    refused(L.load().gymhip_action_log_prob(HERE, L.TYPE_F32, 2, 8, 12, None, HERE, L.ACT_I32, HERE + log_prob, HERE + entropy, HERE + log_sum, None, 0, None), text)
