@@ -17,7 +17,7 @@ namespace policy {
 constexpr int kBlock = 256;
 constexpr int kWave = 64;
 
-// ---- element types: kVec elements are 16 bytes; loads widen to float, stores round once, to nearest even -------------------------------
+// ---- element types: kVec elements are 16 bytes; loads widen to float, stores round a float to nearest even -----------------------------
 struct F32 {
     using T = float;
     static constexpr int kVec = 4;

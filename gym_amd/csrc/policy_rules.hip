@@ -157,7 +157,8 @@ __device__ inline ProcessRow process_row(const Rules& r, int64_t b) {
     return p;
 }
 
-// z = y / T: of 4 bytes one correctly rounded float division where y is the logit itself; under a penalty or a bias y is a double, divided and rounded once.
+// z = y / T: a correctly rounded float division where y is the logit itself; under a penalty or a bias y is a double, divided and rounded to float32.  2-byte results are
+// rounded twice, to float32 and then to their type: 2^-24 of z more than one rounding, which would take the quotient's remainder along for it.
 template <typename E, bool RULES>
 __global__ void __launch_bounds__(kBlock, RULES ? (sizeof(typename E::T) == 4 ? 5 : 4) : 1) process_kernel(const typename E::T* x, int64_t rows, int64_t width, int64_t stride, Rules r, Tiling t,
                                                          typename E::T* out, int64_t out_stride) {

@@ -1,8 +1,8 @@
 // policy_sample.hip — one action per row from softmax of the ruled logits, and its log-probability.
 //
 // The action is the least column whose running sum of exp(y / T) passes u times the whole sum.  Everything that decides it is in double: two
-// neighbouring columns of a flat row of 2^17 lie 8e-6 of the sum apart, about what float32 sums of them are off by, and the same logits must
-// give the same action however the row is laid out and split.  Doubles run at the rate of floats here (30e12 a second, measured), the
+// neighbouring columns of a flat row of 2^17 lie 8e-6 of the sum apart, about what float32 sums of them are off by, and the same logits are to
+// give the same action however the row is laid out and split: they do but for levels within about 1e-13 of the sum of a border (the weights' 4e-14).  Doubles run at the rate of floats here (30e12 a second, measured), the
 // exponential is the 14 instructions of exp2_double, and a double's range lets one pass do without the maximum.
 #include "policy_common.h"
 

@@ -1,8 +1,9 @@
 // policy_score.hip — log-probability and entropy of given actions under the ruled logits: one pass over the logits with a running maximum.
 //
 // With y the logit after penalties and bias, m the greatest y so far, t = (y - m) log2 e / T and w = 2^t:  S = sum w, D = sum w t,
-// log_prob = (y_a - m) / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to y - m, not to y); a lane adds up
-// at most 32 of them before it goes on in double.  m is the same for a wave, so that the sums hardly ever have to be brought to a new one: a few times in
+// log_prob = (y_a - m) / T - ln S, entropy = ln 2 (log2 S - D / S).  t and w are float32 (their errors are relative to y - m, not to y).  Longer
+// rows: a lane adds up the 4 or 8 columns of a vector (or one counted column) in float32 and goes on in double.  Rows in registers: a lane's 2 to 8 columns and then up to 64
+// lanes in pairs, 512 terms at most, all in float32, 13 roundings deep.  m is the same for a wave, so that the sums hardly ever have to be brought to a new one: a few times in
 // a row, by the logarithm of its length.  8.5 vector instructions a column, of the 16 that 2-byte logits leave time for at the memory's rate.
 #include "policy_common.h"
 

@@ -337,7 +337,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
 };
 }  // namespace detail
 
-// z of the logits, rounded once to their type.  Differentiable in the logits.
+// z of the logits, rounded to float32 and from there to their type.  Differentiable in the logits.
 inline at::Tensor processLogits(const at::Tensor& logits, const LogitRules* rules = nullptr) {
     const at::Tensor x = detail::ready(logits, "logits");
     const detail::BoundPtr b = detail::bind(rules, x);

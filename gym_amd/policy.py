@@ -88,9 +88,9 @@ def _rules(rules):
 
 
 def process_logits(logits: torch.Tensor, rules: LogitRules | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """z (LogitRules) of logits [rows, width], rounded once to their type.  Differentiable in the logits.  `out` (not under autograd) may
-    be the logits themselves, or memory that shares no element with them or the rules' tensors (other columns of the same
-    buffer, say).  It changes in place: a backward pass that has saved it raises."""
+    """z (LogitRules) of logits [rows, width], rounded to float32 and from there to their type.  Differentiable in the logits.  `out` (not
+    under autograd) may be the logits themselves, or memory that shares no element with them or the rules' tensors (other columns of the
+    same buffer, say).  It changes in place: a backward pass that has saved it raises."""
     if out is None:
         return _ext.process_logits(logits, _rules(rules))
     _ext.process_logits_into(logits, _rules(rules), out)

@@ -353,7 +353,8 @@ int gymhip_host_env_post_step(int64_t n, const float* reward_in, const uint8_t* 
  * The policy's end of the VecEnv loop: logits to actions, their scores with gradients, dropout.  NO COUNTERPART IN THE REFERENCE
  * (its trainer is outside the repository; VecEnv::step takes finished actions, base.h:56-63).  Stateless: every pointer is device
  * memory of the CURRENT device, calls enqueue on `stream`, allocate nothing and may be recorded into a HIP graph; two calls at once
- * need two workspaces.  Results of a row each must lie neither in the logits nor in each other (GYMHIP_EINVAL).  rows = 0 is allowed and does nothing, width = 0 is rows that allow nothing; either way the rules' pointers are not looked at.
+ * need two workspaces.  Results of a row each must lie neither in the logits nor in each other (GYMHIP_EINVAL).  rows = 0 is allowed
+ * and does nothing, width = 0 is rows that allow nothing; either way the rules' pointers are not looked at.
  * ==================================================================================================================== */
 enum { GYMHIP_TYPE_F32 = 0, GYMHIP_TYPE_F16 = 1, GYMHIP_TYPE_BF16 = 2 };
 /* The widest row of logits or features.  Offsets are 64-bit: rows x stride is not limited. */
@@ -395,16 +396,18 @@ typedef struct gymhip_random_keys {
     const int64_t *rows, *steps;
 } gymhip_random_keys;
 
-/* z of `logits` [rows][width] (type, element stride between rows) rounded once to the same type.  `out` may be `logits` itself (same
- * stride) or lie between its rows (same stride, no element in common); any other overlap of the two is GYMHIP_EINVAL.  What the rules point to must
- * not be written by the call. */
+/* z of `logits` [rows][width] (type, element stride between rows), rounded to float32 and for the 2-byte types from there
+ * to the type: off by half a step of the type and, of those, half a step of float32 at most.  `out` may be `logits` itself (same
+ * stride) or lie between its rows (same stride, no element in common); any other overlap of the two is GYMHIP_EINVAL.  What the
+ * rules point to must not be written by the call. */
 int gymhip_process_logits(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules, void* out,
                           int64_t out_stride, void* stream);
 /* d(logits) from d(z): 0 where the mask's bit is 0. */
 int gymhip_process_logits_backward(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
                                    const void* grad_out, int64_t grad_out_stride, void* grad_in, int64_t grad_in_stride, void* stream);
 /* One action per row from softmax(z), and its log-probability: the least v whose running sum of exp(z - max z) passes u times the whole
- * sum, u in (0, 1) from `keys`.  Decided in double precision, so that the action does not hang on how the row is split or summed.
+ * sum, u in (0, 1) from `keys`.  Sums are in double precision (each weight to 4e-14 of itself), so that how
+ * the row is split or summed matters to an action only where the level lies within about 1e-13 of the sum of a border.
  * A row in which nothing is allowed (or every z is -inf) gives action -1 and log-probability -inf; one that holds a NaN or +inf among
  * its allowed z gives -1 and NaN.  workspace: gymhip_sample_workspace_bytes(rows, width) bytes, 16-B aligned, contents free. */
 size_t gymhip_sample_workspace_bytes(int64_t rows, int64_t width);
