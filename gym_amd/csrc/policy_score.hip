@@ -56,7 +56,8 @@ __device__ inline void add_cols(Run& run, const Y* y, double k2) {
         if (nan) run.s = NAN;
         return;
     }
-    const float k = finite(k2), m = (float)run.m;
+    // (below all floats, where a penalty has taken the type's lowest value: no float but -inf is under it, and -inf less -inf must not come up)
+    const float k = finite(k2), m = __builtin_fmaxf((float)run.m, -3.4028235e38f);
     const float off = LOGITS || m == (float)INFINITY || run.m == (double)m ? 0.f : finite(((double)m - run.m) * __builtin_fmin(k2, 3e38));
     float s = 0, d = 0;
 #pragma unroll

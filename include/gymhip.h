@@ -416,7 +416,7 @@ int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t wi
 /* log softmax(z)[action] and the entropy of softmax(z), float32 per row, and for the backward call alone log_sum, double [rows][2]: the greatest
  * of a row's logits (before the temperature) and the logarithm of the sum of exp(z - max z), apart so that a row of
  * the type's lowest values keeps the latter.  An action
- * that is not allowed or outside [0, width) has -inf, and no gradient; a row in which nothing is allowed has -inf, entropy 0 and no
+ * that is not allowed or outside [0, width) has -inf, and one of -inf (also where float32 holds nothing so low) no gradient; a row in which nothing is allowed has -inf, entropy 0 and no
  * gradient.  workspace as above. */
 size_t gymhip_action_log_prob_workspace_bytes(int64_t rows, int64_t width);
 int gymhip_action_log_prob(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
