@@ -115,7 +115,8 @@ def sample_actions(logits: torch.Tensor, rules: LogitRules | None = None, *, see
 def action_log_prob(logits: torch.Tensor, actions: torch.Tensor, rules: LogitRules | None = None):
     """(log softmax(z)[action], entropy of softmax(z)), float32 [rows] each, for logits [rows, width] and actions int32 / int64 [rows].
     Differentiable in the logits.  An action that is not allowed, or outside [0, width), has -inf, and one of -inf (also where float32 holds
-    nothing so low) hands no gradient back through its log-probability; a row with nothing allowed has -inf, entropy 0 and no gradient."""
+    nothing so low) hands no gradient back through its log-probability; a row with nothing allowed has -inf, entropy 0 and no gradient, one with a NaN or +inf among its allowed z NaN for
+    both and in its gradient, whatever the action."""
     return _ext.action_log_prob(logits, actions, _rules(rules))
 
 

@@ -417,7 +417,9 @@ int gymhip_sample_actions(const void* logits, int type, int64_t rows, int64_t wi
  * of a row's logits (before the temperature) and the logarithm of the sum of exp(z - max z), apart so that a row of
  * the type's lowest values keeps the latter.  An action
  * that is not allowed or outside [0, width) has -inf, and one of -inf (also where float32 holds nothing so low) no gradient; a row in which nothing is allowed has -inf, entropy 0 and no
- * gradient.  workspace as above. */
+ * gradient; one that holds a NaN or +inf among its allowed z has NaN for both, whatever the action.  In float32 beside the logits'
+ * differences: for temperatures below 5e-39 1 / T counts as 3e38 there and in the gradient (logits less than 1e-36 apart notice), and
+ * differences past 3.4e38 count as infinite (temperatures above 1e30 notice).  workspace as above. */
 size_t gymhip_action_log_prob_workspace_bytes(int64_t rows, int64_t width);
 int gymhip_action_log_prob(const void* logits, int type, int64_t rows, int64_t width, int64_t stride, const gymhip_logit_rules* rules,
                            const void* actions, int action_dtype, float* log_prob, float* entropy, double* log_sum, void* workspace,
