@@ -28,7 +28,8 @@ struct Error : std::runtime_error { using std::runtime_error::runtime_error; };
 
 namespace detail {
 
-inline void require(bool ok, const std::string& what) { if (!ok) throw std::invalid_argument(what); }
+[[noreturn]] inline void refuse(const std::string& what) { throw std::invalid_argument(what); }
+inline void require(bool ok, const std::string& what) { if (!ok) refuse(what); }
 inline void check(int rc, const char* what) {
     if (rc != GYMHIP_OK) throw Error(std::string(what) + " failed (code " + std::to_string(rc) + "): " + gymhip_last_error());
 }
@@ -53,11 +54,11 @@ inline void noTangent(const at::Tensor& x, const char* what) {
 
 // derived: the result has a derivative in x.
 inline at::Tensor ready(const at::Tensor& x, const char* what, bool derived = true) {
-    require(x.dim() == 2, std::string(what) + " must be a 2-D tensor [rows, width]");
-    require(typeOf(x.scalar_type()) >= 0, std::string(what) + " must be float32, float16 or bfloat16, got " + at::toString(x.scalar_type()));
+    if (x.dim() != 2) refuse(std::string(what) + " must be a 2-D tensor [rows, width]");
+    if (typeOf(x.scalar_type()) < 0) refuse(std::string(what) + " must be float32, float16 or bfloat16, got " + at::toString(x.scalar_type()));
     if (derived) noTangent(x, what);
     if (!x.is_cuda()) throw Error(std::string(what) + " is on " + x.device().str() + ": the policy kernels run on the GPU and have no CPU fallback");
-    require(x.size(1) <= GYMHIP_POLICY_MAX_WIDTH, std::string(what) + ": at most 2^24 columns, got " + std::to_string(x.size(1)));
+    if (x.size(1) > GYMHIP_POLICY_MAX_WIDTH) refuse(std::string(what) + ": at most 2^24 columns, got " + std::to_string(x.size(1)));
     return rowwise(x);
 }
 
@@ -124,10 +125,10 @@ private:
         if (v.rows.defined()) return;
         // as the kernels take it: a number too small for float32 must not turn into the 0 that stands for something else
         const bool fits = std::abs(v.number) <= std::numeric_limits<float>::max(), positive_f = (float)v.number > 0;
-        std::ostringstream got;
-        got << v.number;
-        detail::require(fits && (!positive || positive_f) && (!not_negative || positive_f || v.number == 0),
-                        std::string(name) + " must be a finite float32" + (positive ? ", and positive" : not_negative ? ", and not negative" : "") + "; got " + got.str());
+        if (fits && (!positive || positive_f) && (!not_negative || positive_f || v.number == 0)) return;
+        std::ostringstream what;
+        what << name << " must be a finite float32" << (positive ? ", and positive" : not_negative ? ", and not negative" : "") << "; got " << v.number;
+        detail::refuse(what.str());
     }
 };
 
@@ -363,10 +364,11 @@ inline void processLogitsInto(const at::Tensor& logits, const LogitRules* rules,
 // where both are given, which is a change of them in place.
 inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits, const LogitRules* rules, const Keys& keys, at::Tensor actions = {},
                                                         at::Tensor log_prob = {}) {
-    detail::require(actions.defined() == log_prob.defined(), "out needs both actions and log_prob, or neither");
+    if (actions.defined() != log_prob.defined()) detail::refuse("out needs both actions and log_prob, or neither");
+    const bool given = actions.defined();
     const at::Tensor x = detail::ready(logits, "logits", false);
     const int64_t n = x.size(0), width = x.size(1);
-    if (actions.defined()) {
+    if (given) {
         detail::side(actions, "out.actions", x.device(), {at::kInt}, {{n}});
         detail::side(log_prob, "out.log_prob", x.device(), {at::kFloat}, {{n}});
         detail::require(actions.is_contiguous() && log_prob.is_contiguous(), "out tensors must be contiguous");
@@ -378,8 +380,10 @@ inline std::tuple<at::Tensor, at::Tensor> sampleActions(const at::Tensor& logits
     const detail::BoundKeys k(keys, n, x.device());
     const size_t bytes = gymhip_sample_workspace_bytes(n, width);
     const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : at::Tensor();
-    detail::written(actions);
-    detail::written(log_prob);
+    if (given) {
+        detail::written(actions);
+        detail::written(log_prob);
+    }
     const c10::OptionalDeviceGuard guard(x.device());
     detail::check(gymhip_sample_actions(x.data_ptr(), detail::typeOf(x.scalar_type()), n, width, x.stride(0), b->ptr(), &k.c, actions.data_ptr<int32_t>(),
                                         log_prob.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, detail::stream(x)), "gymhip_sample_actions");
@@ -402,7 +406,7 @@ inline std::tuple<at::Tensor, at::Tensor> actionLogProb(const at::Tensor& logits
 // x [rows, width] with each element 0 with probability p (to 16 bits), else multiplied by 65536 / (65536 - round(65536 p)).  Differentiable in x.
 inline at::Tensor dropout(const at::Tensor& x_, double p, const Keys& keys) {
     const at::Tensor x = detail::ready(x_, "x");
-    detail::require(p >= 0 && p < 1 && std::nearbyint(65536 * p) <= 65535, "p must lie in [0, 1) and round to less than 65536 / 65536, got " + std::to_string(p));
+    if (!(p >= 0 && p < 1 && std::nearbyint(65536 * p) <= 65535)) detail::refuse("p must lie in [0, 1) and round to less than 65536 / 65536, got " + std::to_string(p));
     auto k = c10::make_intrusive<detail::BoundKeys>(keys, x.size(0), x.device());
     return detail::graded(x_) ? detail::DropoutFunction::apply(x_, p, k) : detail::drop(x, p, *k);
 }
