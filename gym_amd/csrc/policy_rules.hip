@@ -134,7 +134,7 @@ struct ProcessRow : Row {
     // y / T on its way to a float: divided, or for 2-byte results, whose rounding hides 1e-16, multiplied by the reciprocal (2,048 x 49,999 bf16 under all rules: 208 -> 180 us).
     template <typename E>
     __device__ double over(double y) const { return sizeof(typename E::T) == 2 ? y * inv_temp : divided(y, temp, inv_temp); }
-    // (RULES: where the vector unit is the bound; without them the float division is as fast, 79 and 86 us of 2,048 x 49,999 bf16.)
+    // (RULES: where vector instructions cost time; without them the float division is as fast, 79 and 86 us of 2,048 x 49,999 bf16.)
     template <typename E, bool RULES, int C>
     __device__ void over_cols(float* v) const {
         if (undivided) return;
