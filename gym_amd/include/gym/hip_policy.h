@@ -95,7 +95,9 @@ struct PerRow {
     double number = 0;
     at::Tensor rows;
     PerRow(double n) : number(n) {}
-    PerRow(at::Tensor t) : rows(std::move(t)) {}
+    PerRow(at::Tensor t) : rows(std::move(t)) {
+        if (!rows.defined()) detail::refuse("a number per row is an undefined tensor");   // it would stand for the number 0: a greedy temperature
+    }
 };
 
 // What is done to a row's logits before anything is chosen or scored: gymhip_logit_rules in tensors.
